@@ -17,9 +17,12 @@ LIBNAME = 'libopenpvsg_hip.so'
 ARCH = 'gfx950'
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 CFLAGS = ['--offload-arch=' + ARCH, '-O3', '-std=c++17', '-fPIC',
-          '-Wall', '-Wno-unused-function']
-# per-file additions.  winograd3x3: packed-f32 VALU (v_pk_add_f32 built by the SLP vectoriser, with the v_movs that feed
-# it) beside f32 MFMAs costs issue slots the scalar adds do not.
+          '-Wall', '-Wno-unused-function',
+          # no packed-f32 VALU (v_pk_add / mul / fma_f32): the vectoriser makes them from ordinary float code, and beside the
+          # MFMAs some of their forms have given wrong results on this part without an error (tests/test_mfma_hazard.py)
+          '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+# per-file additions.  winograd3x3: what the SLP vectoriser builds (with the v_movs that feed it) beside f32 MFMAs costs issue
+# slots the scalar adds do not.
 EXTRA_CFLAGS = {'winograd3x3.hip': ['-fno-slp-vectorize']}
 
 
