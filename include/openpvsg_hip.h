@@ -642,6 +642,59 @@ int pvsg_bottleneck_tail_f16x2(const float* mid, const void* w3_packed, const fl
                                float* y, float* y_stride2, const void* w1n_packed, const float* scale1n, const float* shift1n,
                                float* mid_next, int B, int Cmid, int Cout, int Cnext, int H, int W, uint32_t* overflow, void* stream);
 
+/* ---- paged key/value cache: live video --------------------------------------------------------
+ * The reference re-runs its temporal encoder over every frame so far (models/relation_head/transformer.py:26-56 takes the whole
+ * (P, T, C) block); with these a call projects only its new frames, appends their keys and values, and attends over the cache.
+ *
+ * A pool holds K and V as (num_pages, heads, page_size, dim): dim dense, the first three axes with strides in ELEMENTS, the same
+ * for K and V and multiples of 16 bytes; base addresses 16-byte aligned.  page_size: a power of two in [8, 65536]; dim: a multiple of 16 up
+ * to 256.  type: of the stored elements.  The 8-bit types hold x / s with one f32 scale s per row, k_scale / v_scale
+ * (num_pages, heads, page_size): slots dense, page / head strides multiples of 4, bases 16-byte aligned; NULL otherwise.
+ * Position p of sequence b is slot p % page_size of page table[b][p / page_size] (table: (B, table_width) int32 rows table_stride apart,
+ * table_width * page_size <= 2^30).  lens[b] (int32, device) counts the cached positions INCLUDING this call's new ones; of the T new
+ * rows per sequence the first n_b = min(T, lens[b], new_lens[b]) are real (new_lens NULL: T), at positions lens[b] - n_b + t.
+ * Lengths and page ids live on the device, so they are checked there: a page id outside the pool, or a length past the table, is
+ * never followed -- such rows are not written / read as zero / not attended to, and a bit of *faults (may be NULL) is set:
+ * 1 append, 2 read, 4 attention.
+ * Pages that a sequence appends to belong to it alone; pages that are only read may be in several rows of the table. */
+#define PVSG_TYPE_F32 0
+#define PVSG_TYPE_BF16 1
+#define PVSG_TYPE_F16 2
+#define PVSG_TYPE_E4M3 3
+#define PVSG_TYPE_I8 4
+typedef struct pvsg_kv_pages {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  long long page_stride, head_stride, slot_stride;
+  long long scale_page_stride, scale_head_stride;
+  int num_pages, heads, page_size, dim, type;
+  int* faults;
+} pvsg_kv_pages;
+/* New rows k, v (B, T, heads, dim) of row_type (F32, BF16, F16; dim dense, strides in elements, the same for both, multiples of 16
+ * bytes, bases 16-byte aligned) into the pool, rounded to its type once: to nearest even; 8-bit: with a = max|x| of the row,
+ * s = max(a * f32(1/448) or a * f32(1/127), 2^-126), code = x / s.  A row that holds a NaN or infinity reads back as NaN. */
+int pvsg_kv_append(const pvsg_kv_pages* pages, const void* k, const void* v, int row_type, long long seq_stride,
+                   long long token_stride, long long head_stride, const int* table, long long table_stride, int table_width,
+                   const int* lens, const int* new_lens, int B, int T, void* stream);
+/* Positions start .. start+length-1 of every sequence as dense (B, length, heads, dim) k_out, v_out of out_type (F32, BF16, F16;
+ * 16-byte aligned): code * s, rounded once; zero rows at positions >= lens[b]. */
+int pvsg_kv_read(const pvsg_kv_pages* pages, void* k_out, void* v_out, int out_type, const int* table, long long table_stride,
+                 int table_width, const int* lens, int B, int start, int length, void* stream);
+/* Attention of the new tokens over the cache: q (B, T, q_heads, dim) and out, dense in dim, of row_type; q_heads a multiple of the
+ * pool's heads (query head j reads key head j / (q_heads / heads)); T <= 32.  Pools: of row_type, or 8-bit; with row_type F32 any.
+ * Row t of sequence b sees positions p < lens[b], with causal != 0 only p <= lens[b] - n_b + t, and with padding (bool bytes,
+ * (B, padding_width) rows padding_stride apart, nonzero = ignored) only p < padding_width with a zero there.  softmax(scale * q.k) v in f32, rounded
+ * once; a row that sees nothing, or past n_b, is zero.  What a row does not see does not reach it, NaN and infinities included.
+ * max_len: the longest cache to plan for (0: what the table holds); longer ones are computed all the same.
+ * splits: how many workgroups share the cache of one (sequence, key head), from pvsg_paged_attention_splits; > 1 needs
+ * B * T * q_heads * splits * (dim + 2) floats of scratch in `workspace` (16-byte aligned, no initialisation). */
+int pvsg_paged_attention_splits(int B, int T, int q_heads, int kv_heads, int dim, int type, long long max_len);
+int pvsg_paged_attention(const pvsg_kv_pages* pages, const void* q, long long q_seq_stride, long long q_token_stride,
+                         long long q_head_stride, void* out, int row_type, const int* table, long long table_stride, int table_width,
+                         const int* lens, const int* new_lens, const uint8_t* padding, long long padding_stride, int padding_width,
+                         int B, int T, int q_heads, float scale, int causal, long long max_len, int splits, void* workspace,
+                         void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -48,6 +48,13 @@ class RelationTail(ctypes.Structure):
         ('dim', _i), ('num_relations', _i), ('eps', _f)]
 
 
+class KvPages(ctypes.Structure):
+    """pvsg_kv_pages (include/openpvsg_hip.h)"""
+    _fields_ = [(n, ctypes.c_void_p) for n in ('k', 'v', 'k_scale', 'v_scale')] + [(n, _ll) for n in (
+        'page_stride', 'head_stride', 'slot_stride', 'scale_page_stride', 'scale_head_stride')] + [
+        (n, _i) for n in ('num_pages', 'heads', 'page_size', 'dim', 'type')] + [('faults', ctypes.c_void_p)]
+
+
 # name -> argtypes; must list every function include/openpvsg_hip.h declares
 # (tests/test_capi.py cross-checks this table against the header).
 SIGNATURES = {
@@ -143,13 +150,18 @@ SIGNATURES = {
     'pvsg_stem7x7_f16x2_matrix': [_c_f, _c_f, _c_f],
     'pvsg_stem7x7_f16x2_bn_relu_pool': [_c_f] * 5 + [_i, _i, _i, _c_f, _c_f],
     'pvsg_conv3x3s2_affine': [_c_f] * 5 + [_i] * 6 + [_c_f],
+    'pvsg_kv_append': [ctypes.POINTER(KvPages), _c_f, _c_f, _i, _ll, _ll, _ll, _c_f, _ll, _i, _c_f, _c_f, _i, _i, _c_f],
+    'pvsg_kv_read': [ctypes.POINTER(KvPages), _c_f, _c_f, _i, _c_f, _ll, _i, _c_f, _i, _i, _i, _c_f],
+    'pvsg_paged_attention_splits': [_i] * 6 + [_ll],
+    'pvsg_paged_attention': [ctypes.POINTER(KvPages), _c_f, _ll, _ll, _ll, _c_f, _i, _c_f, _ll, _i, _c_f, _c_f, _c_f, _ll, _i, _i, _i,
+                             _i, _f, _i, _ll, _i, _c_f, _c_f],
 }
 # entry points that return a value instead of a status code
 VALUE_RETURNING = ('pvsg_xattn_num_splits', 'pvsg_gemm_bf16x3_packed_elems', 'pvsg_gemm_f16x2_packed_elems',
                    'pvsg_minvis_chain_workspace_bytes', 'pvsg_reconsdot_workspace_bytes', 'pvsg_rle_counts_to_chars',
                    'pvsg_decoder_rows_post_workspace_bytes', 'pvsg_tube_index_table_words', 'pvsg_conv1x1_stats_chunks',
                    'pvsg_conv3x3_stats_chunks', 'pvsg_rel_tail_workspace_bytes', 'pvsg_conv_slices', 'pvsg_rle_segments',
-                   'pvsg_rows_f16x2_packed_floats')
+                   'pvsg_rows_f16x2_packed_floats', 'pvsg_paged_attention_splits')
 
 _lib = None
 
@@ -199,7 +211,7 @@ def load():
 # capture warm-ups do), but never run on two at once: a launch on stream S while the stream that carried the previous launches
 # still has work pending is an error when either side is a 16-bit-MFMA kernel.  PVSG_MULTI_STREAM=allow switches the check off
 # (measurements of the effect itself).
-_MFMA16 = ('bf16x3', 'f16x2', 'masked_xattn')
+_MFMA16 = ('bf16x3', 'f16x2', 'masked_xattn', 'paged_attention')
 _MFMA16_NAMES = frozenset(n for n in SIGNATURES if any(k in n for k in _MFMA16))
 # Per DEVICE: [stream handle of the previous launch there, has that stream run a 16-bit-MFMA kernel since it took over].
 # Kernels on different devices cannot co-reside, so a process that drives two GPUs (or two threads, one GPU each) alternates

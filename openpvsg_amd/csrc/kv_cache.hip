@@ -1,0 +1,277 @@
+// Writing a paged key/value pool (quantising on the way) and reading it back dense.
+//
+// Both are one pass over the rows and bound by memory: a row is 2 * dim elements in one type in, the same in another out, and
+// a scale.  A lane holds 8 elements of a row's K and of its V (16-byte accesses on the 16-bit side), so a row is next_pow2(dim/8)
+// lanes: 16 at dim 128, four rows to a wave, and the row's maximum needs log2 of that in lane exchanges and no LDS.
+#include "kv_pages.h"
+
+namespace pvsg {
+
+int kv_check_pages(const char* who, const pvsg_kv_pages* p, const int* table, long long table_stride, int table_width, const int* lens, int B) {
+  PVSG_REQUIRE(p && p->k && p->v && table && lens, "%s: null pointer", who);
+  PVSG_REQUIRE(p->type >= KV_F32 && p->type <= KV_I8, "%s: pool type %d", who, p->type);
+  PVSG_REQUIRE(p->num_pages > 0 && p->heads > 0 && p->heads <= 65535, "%s: %d pages, %d heads", who, p->num_pages, p->heads);
+  PVSG_REQUIRE(p->page_size >= 8 && p->page_size <= 65536 && (p->page_size & (p->page_size - 1)) == 0, "%s: page_size %d is no power of two in [8, 65536]", who, p->page_size);
+  PVSG_REQUIRE(p->dim >= 16 && p->dim <= 256 && p->dim % 16 == 0, "%s: dim %d is no multiple of 16 up to 256", who, p->dim);
+  const long long unit = 16 / kv_bytes(p->type);
+  PVSG_REQUIRE(p->page_stride % unit == 0 && p->head_stride % unit == 0 && p->slot_stride % unit == 0 && (((uintptr_t)p->k | (uintptr_t)p->v) & 15) == 0,
+               "%s: the pool's rows are not 16-byte aligned", who);
+  PVSG_REQUIRE(p->page_stride >= 0 && p->head_stride >= 0 && p->slot_stride >= p->dim, "%s: bad pool strides", who);
+  if (kv_scaled(p->type)) {
+    PVSG_REQUIRE(p->k_scale && p->v_scale, "%s: an 8-bit pool needs its scales", who);
+    PVSG_REQUIRE(p->scale_page_stride % 4 == 0 && p->scale_head_stride % 4 == 0 && (((uintptr_t)p->k_scale | (uintptr_t)p->v_scale) & 15) == 0,
+                 "%s: the scales are not 16-byte aligned", who);
+  }
+  PVSG_REQUIRE(B >= 0 && B <= 65535, "%s: %d sequences (at most 65535)", who, B);
+  PVSG_REQUIRE(table_width > 0 && table_stride >= 0 && (long long)table_width * p->page_size <= (1ll << 30), "%s: table of %d pages of %d (positions stay below 2^30)", who,
+               table_width, p->page_size);
+  return PVSG_OK;
+}
+
+struct KvAppend {
+  pvsg_kv_pages p;
+  const unsigned char *k, *v;
+  long long seq_stride, token_stride, head_stride;   // bytes
+  const int* table;
+  long long table_stride;
+  const int *lens, *new_lens;
+  int width, T, page_shift, lanes_shift;
+};
+
+constexpr float KV_TINY = 1.17549435e-38f;           // 2^-126: keeps x / s finite where the row is all zeros or denormal
+
+// eight f32 -> the row's stored words; `s` is the 8-bit types' scale.  x / s is the correctly rounded quotient: a multiplication
+// by 1/s would put values that lie next to a border between two codes on its other side.
+template <int CT>
+__device__ __forceinline__ void kv_encode8(const float* x, float s, unsigned* w) {
+  if constexpr (CT == KV_F32) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = __builtin_bit_cast(unsigned, x[i]);
+  } else if constexpr (CT == KV_BF16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = kv_pack_bf16(x[2 * i], x[2 * i + 1]);
+  } else if constexpr (CT == KV_F16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = kv_pack_f16(x[2 * i], x[2 * i + 1]);
+  } else if constexpr (CT == KV_E4M3) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i] / s, x[4 * i + 1] / s, 0, false);
+      w[i] = (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2] / s, x[4 * i + 3] / s, lo, true);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      unsigned u = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // |x / s| <= 127 * (1 + 2^-22), so rounding stays in range; x / s of a row with a NaN or infinity is 0 or NaN, both code 0,
+        // which its scale reads back as NaN
+        const float r = rintf(x[4 * i + j] / s);
+        u |= ((unsigned)(r == r ? (int)r : 0) & 255u) << (8 * j);
+      }
+      w[i] = u;
+    }
+  }
+}
+
+template <int RT, int CT>
+__device__ __forceinline__ void kv_append_row(const unsigned (&raw)[kv_bytes(RT) * 2], unsigned char* dst, float* scale, int lanes, bool live, bool lane0, bool in_dim) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = kv_elem<RT>(raw, i);
+  float s = 1.f;
+  if constexpr (kv_scaled(CT)) {
+    // the maximum of the magnitudes' bits: a NaN is above infinity is above every number, so a row that holds one has a scale
+    // of NaN or infinity
+    unsigned a = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = max(a, __builtin_bit_cast(unsigned, x[i]) & 0x7fffffffu);
+    for (int o = lanes >> 1; o >= 1; o >>= 1) a = max(a, (unsigned)__shfl_xor((int)a, o));
+    const float m = __builtin_bit_cast(float, a);
+    s = m * (CT == KV_E4M3 ? 1.f / 448.f : 1.f / 127.f);
+    s = s < KV_TINY ? KV_TINY : s;                     // a NaN stays
+    if (live && lane0) *scale = s;
+  }
+  if (live && in_dim) {
+    unsigned w[kv_bytes(CT) * 2];
+    kv_encode8<CT>(x, s, w);
+    if constexpr (CT == KV_F32) {
+      kv_store<16>(dst, w);
+      kv_store<16>(dst + 16, w + 4);
+    } else {
+      kv_store<kv_bytes(CT) * 8>(dst, w);
+    }
+  }
+}
+
+template <int RT, int CT>
+__global__ __launch_bounds__(256) void kv_append_kernel(const KvAppend a) {
+  constexpr int RB = kv_bytes(RT), CB = kv_bytes(CT);
+  const int b = blockIdx.y;
+  const int lanes = 1 << a.lanes_shift;
+  const int sub = threadIdx.x & (lanes - 1);
+  const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) >> a.lanes_shift;
+  const int h = (int)(r % a.p.heads);
+  const long long t = r / a.p.heads;
+  const KvSpan span = kv_span(a.lens, a.new_lens, b, a.T, a.width << a.page_shift);
+  bool live = t < span.fresh;
+  const int pos = live ? span.len - span.fresh + (int)t : 0;
+  int page = 0;
+  if (live) {
+    page = pos < span.there ? a.table[(long long)b * a.table_stride + (pos >> a.page_shift)] : -1;
+    if ((unsigned)page >= (unsigned)a.p.num_pages) {
+      live = false;
+      page = 0;
+      if (sub == 0) kv_fault(a.p.faults, 1);
+    }
+  }
+  const bool in_dim = 8 * sub < a.p.dim;
+  unsigned kr[RB * 2] = {}, vr[RB * 2] = {};
+  if (live && in_dim) {
+    const long long src = b * a.seq_stride + t * a.token_stride + h * a.head_stride + sub * (8 * RB);
+    kv_load<16>(kr, a.k + src);
+    kv_load<16>(vr, a.v + src);
+    if constexpr (RB == 4) {
+      kv_load<16>(kr + 4, a.k + src + 16);
+      kv_load<16>(vr + 4, a.v + src + 16);
+    }
+  }
+  const int slot = pos & (a.p.page_size - 1);
+  const long long dst = ((long long)page * a.p.page_stride + (long long)h * a.p.head_stride + (long long)slot * a.p.slot_stride + 8 * sub) * CB;
+  const long long sc = (long long)page * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + slot;
+  kv_append_row<RT, CT>(kr, static_cast<unsigned char*>(a.p.k) + dst, a.p.k_scale + sc, lanes, live, sub == 0, in_dim);
+  kv_append_row<RT, CT>(vr, static_cast<unsigned char*>(a.p.v) + dst, a.p.v_scale + sc, lanes, live, sub == 0, in_dim);
+}
+
+struct KvRead {
+  pvsg_kv_pages p;
+  unsigned char *k, *v;
+  const int* table;
+  long long table_stride;
+  const int* lens;
+  int width, start, length, page_shift, lanes_shift;
+};
+
+template <int RT, int CT>
+__global__ __launch_bounds__(256) void kv_read_kernel(const KvRead a) {
+  constexpr int RB = kv_bytes(RT), CB = kv_bytes(CT);
+  const int b = blockIdx.y;
+  const int sub = threadIdx.x & ((1 << a.lanes_shift) - 1);
+  const long long r = ((long long)blockIdx.x * 256 + threadIdx.x) >> a.lanes_shift;
+  const int h = (int)(r % a.p.heads);
+  const long long t = r / a.p.heads;
+  if (t >= a.length || 8 * sub >= a.p.dim) return;
+  const KvSpan span = kv_span(a.lens, nullptr, b, 0, a.width << a.page_shift);
+  const long long pos = a.start + t;
+  unsigned kw[CB * 2] = {}, vw[CB * 2] = {};
+  float ks = 0.f, vs = 0.f;
+  if (pos < span.len) {
+    const int page = pos < span.there ? a.table[(long long)b * a.table_stride + (pos >> a.page_shift)] : -1;
+    if ((unsigned)page < (unsigned)a.p.num_pages) {
+      const int slot = (int)pos & (a.p.page_size - 1);
+      const long long src = ((long long)page * a.p.page_stride + (long long)h * a.p.head_stride + (long long)slot * a.p.slot_stride + 8 * sub) * CB;
+      constexpr int N = CB == 4 ? 16 : CB * 8;
+      kv_load<N>(kw, static_cast<const unsigned char*>(a.p.k) + src);
+      kv_load<N>(vw, static_cast<const unsigned char*>(a.p.v) + src);
+      if constexpr (CB == 4) {
+        kv_load<16>(kw + 4, static_cast<const unsigned char*>(a.p.k) + src + 16);
+        kv_load<16>(vw + 4, static_cast<const unsigned char*>(a.p.v) + src + 16);
+      }
+      if constexpr (kv_scaled(CT)) {
+        const long long sc = (long long)page * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + slot;
+        ks = a.p.k_scale[sc], vs = a.p.v_scale[sc];
+      }
+    } else if (sub == 0) {
+      kv_fault(a.p.faults, 2);
+    }
+  }
+  const long long dst = (((long long)b * a.length * a.p.heads + r) * a.p.dim + 8 * sub) * RB;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const unsigned* w = which ? vw : kw;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = kv_elem<CT>(w, i);
+      if constexpr (kv_scaled(CT)) x[i] *= which ? vs : ks;
+    }
+    unsigned o[RB * 2];
+    kv_encode8<RT>(x, 1.f, o);
+    unsigned char* out = (which ? a.v : a.k) + dst;
+    kv_store<16>(out, o);
+    if constexpr (RB == 4) kv_store<16>(out + 16, o + 4);
+  }
+}
+
+static int kv_log2(int x) {
+  int s = 0;
+  while ((1 << s) < x) ++s;
+  return s;
+}
+
+template <int RT, int CT, class A>
+static void kv_launch(const A& a, dim3 grid, hipStream_t stream) {
+  if constexpr (__is_same(A, KvAppend)) {
+    hipLaunchKernelGGL((kv_append_kernel<RT, CT>), grid, dim3(256), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((kv_read_kernel<RT, CT>), grid, dim3(256), 0, stream, a);
+  }
+}
+template <int RT, class A>
+static void kv_launch(const A& a, dim3 grid, hipStream_t stream) {
+  switch (a.p.type) {
+    case KV_F32: kv_launch<RT, KV_F32>(a, grid, stream); break;
+    case KV_BF16: kv_launch<RT, KV_BF16>(a, grid, stream); break;
+    case KV_F16: kv_launch<RT, KV_F16>(a, grid, stream); break;
+    case KV_E4M3: kv_launch<RT, KV_E4M3>(a, grid, stream); break;
+    default: kv_launch<RT, KV_I8>(a, grid, stream);
+  }
+}
+template <class A>
+static void kv_launch(int row_type, const A& a, dim3 grid, hipStream_t stream) {
+  switch (row_type) {
+    case KV_F32: kv_launch<KV_F32>(a, grid, stream); break;
+    case KV_BF16: kv_launch<KV_BF16>(a, grid, stream); break;
+    default: kv_launch<KV_F16>(a, grid, stream);
+  }
+}
+
+}  // namespace pvsg
+
+extern "C" int pvsg_kv_append(const pvsg_kv_pages* pages, const void* k, const void* v, int row_type, long long seq_stride,
+                              long long token_stride, long long head_stride, const int* table, long long table_stride, int table_width,
+                              const int* lens, const int* new_lens, int B, int T, void* stream) {
+  using namespace pvsg;
+  if (const int rc = kv_check_pages("pvsg_kv_append", pages, table, table_stride, table_width, lens, B)) return rc;
+  PVSG_REQUIRE(k && v, "pvsg_kv_append: null pointer");
+  PVSG_REQUIRE(row_type >= KV_F32 && row_type <= KV_F16, "pvsg_kv_append: row type %d", row_type);
+  const long long rb = kv_bytes(row_type);
+  PVSG_REQUIRE(((seq_stride | token_stride | head_stride) * rb) % 16 == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0, "pvsg_kv_append: rows are not 16-byte aligned");
+  PVSG_REQUIRE(T >= 0, "pvsg_kv_append: %d tokens", T);
+  if (B == 0 || T == 0) return PVSG_OK;
+  KvAppend a{*pages, static_cast<const unsigned char*>(k), static_cast<const unsigned char*>(v), seq_stride * rb, token_stride * rb, head_stride * rb,
+             table, table_stride, lens, new_lens, table_width, T, kv_log2(pages->page_size), kv_log2(pages->dim / 8)};
+  const long long blocks = (((long long)T * pages->heads << a.lanes_shift) + 255) / 256;
+  PVSG_REQUIRE(blocks < (1ll << 31), "pvsg_kv_append: %d tokens of %d heads are too many for one launch", T, pages->heads);
+  kv_launch(row_type, a, dim3((unsigned)blocks, (unsigned)B), static_cast<hipStream_t>(stream));
+  PVSG_LAUNCH_CHECK("pvsg_kv_append");
+  return PVSG_OK;
+}
+
+extern "C" int pvsg_kv_read(const pvsg_kv_pages* pages, void* k_out, void* v_out, int out_type, const int* table, long long table_stride,
+                            int table_width, const int* lens, int B, int start, int length, void* stream) {
+  using namespace pvsg;
+  if (const int rc = kv_check_pages("pvsg_kv_read", pages, table, table_stride, table_width, lens, B)) return rc;
+  PVSG_REQUIRE(k_out && v_out && (((uintptr_t)k_out | (uintptr_t)v_out) & 15) == 0, "pvsg_kv_read: null or misaligned output");
+  PVSG_REQUIRE(out_type >= KV_F32 && out_type <= KV_F16, "pvsg_kv_read: output type %d", out_type);
+  PVSG_REQUIRE(start >= 0 && length >= 0, "pvsg_kv_read: positions %d + %d", start, length);
+  if (B == 0 || length == 0) return PVSG_OK;
+  KvRead a{*pages, static_cast<unsigned char*>(k_out), static_cast<unsigned char*>(v_out), table, table_stride, lens, table_width, start, length,
+           kv_log2(pages->page_size), kv_log2(pages->dim / 8)};
+  const long long blocks = (((long long)length * pages->heads << a.lanes_shift) + 255) / 256;
+  PVSG_REQUIRE(blocks < (1ll << 31), "pvsg_kv_read: %d positions of %d heads are too many for one launch", length, pages->heads);
+  kv_launch(out_type, a, dim3((unsigned)blocks, (unsigned)B), static_cast<hipStream_t>(stream));
+  PVSG_LAUNCH_CHECK("pvsg_kv_read");
+  return PVSG_OK;
+}

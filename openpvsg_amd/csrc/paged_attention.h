@@ -1,0 +1,550 @@
+// Attention of 1..32 new tokens per sequence over a paged key/value pool, split over the cache's length and joined.
+//
+//   o = sum_p softmax(scale * q . k_p) v_p,  one pass over the keys with a running maximum m and sum l per row.
+//
+// The T * (q_heads / kv_heads) query rows that share a key head make 16-row tiles.  A wave walks the cache in tiles of KEYS keys and
+// feeds the matrix cores straight from global memory, with no LDS between: keys are the A operand of S^T = K Q^T (a lane's part of
+// a row is dense in memory), and S^T leaves the pipe with a lane holding 4 keys of one query row -- which is the B operand of
+// O^T = V^T P^T as it stands, so P never moves.  For V^T a lane loads the same columns of several keys and pairs them by
+// byte permutes (16-bit products take 8 keys a lane; f32 products take one, and need no permutes).  Four waves take every
+// fourth tile and meet in LDS at the end; where few rows leave the card idle, `splits` workgroups share a cache and a second
+// kernel joins their (m, l, O).
+//
+// Rounding: 16-bit rows multiply in their own type, exact products in f32 sums; 8-bit codes convert to it exactly and their
+// scales multiply S and P in f32.  P goes to the matrix cores as a 16-bit high part plus a 16-bit rest (one part alone adds an error as
+// large as the rounding of the result itself).  f32 rows run in f32 throughout.
+#pragma once
+#include "kv_pages.h"
+
+namespace pvsg {
+
+struct PagedAttn {
+  pvsg_kv_pages p;
+  const unsigned char* q;
+  unsigned char* out;
+  const int* table;
+  const int *lens, *new_lens;
+  const unsigned char* padding;
+  float *part_o, *part_ml;
+  long long q_seq, q_token, q_head;      // bytes
+  long long table_stride, padding_stride;
+  float scale_log2e;
+  int width, padding_width, page_shift;
+  int B, T, q_heads, group, rows, row_groups, splits, chunk, causal;
+};
+
+constexpr int PA_WAVES = 4;
+constexpr int PA_MAX_CHUNK = 4096;
+constexpr int PA_MAX_T = 32;
+
+// four packed 16-bit words (the 8 elements of one lane of a matrix product's operand)
+template <int MT>
+__device__ __forceinline__ f32x4 pa_mfma16(const unsigned (&a)[4], const unsigned (&b)[4], f32x4 c) {
+  const kv_u32x4 av = {a[0], a[1], a[2], a[3]}, bv = {b[0], b[1], b[2], b[3]};
+  if constexpr (MT == KV_BF16) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(kv_bf16x8, av), __builtin_bit_cast(kv_bf16x8, bv), c, 0, 0, 0);
+  } else {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(kv_f16x8, av), __builtin_bit_cast(kv_f16x8, bv), c, 0, 0, 0);
+  }
+}
+template <int MT>
+__device__ __forceinline__ unsigned pa_pack(float a, float b) {
+  return MT == KV_BF16 ? kv_pack_bf16(a, b) : kv_pack_f16(a, b);
+}
+template <int MT>
+__device__ __forceinline__ float pa_half(unsigned w, int i) {
+  return MT == KV_BF16 ? kv_elem<KV_BF16>(&w, i) : kv_elem<KV_F16>(&w, i);
+}
+// bytes 2i, 2i+1 of an 8-bit word -> a packed 16-bit pair
+template <int MT, int CT>
+__device__ __forceinline__ unsigned pa_widen(unsigned w, bool hi) {
+  if constexpr (CT == KV_E4M3) {
+    if constexpr (MT == KV_BF16) {
+      return __builtin_bit_cast(unsigned, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
+    } else {
+      return __builtin_bit_cast(unsigned, hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
+    }
+  } else {
+    return pa_pack<MT>(kv_elem<KV_I8>(&w, hi ? 2 : 0), kv_elem<KV_I8>(&w, hi ? 3 : 1));
+  }
+}
+
+// maximum / sum over the four 16-lane groups of a wave, in every lane
+__device__ __forceinline__ float pa_max4(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float pa_sum4(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+template <int RT>
+__device__ __forceinline__ void pa_store_row4(unsigned char* out, long long at, const float (&x)[4]) {
+  unsigned w[4];
+  if constexpr (RT == KV_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __builtin_bit_cast(unsigned, x[i]);
+    kv_store<16>(out + at * 4, w);
+  } else {
+    w[0] = pa_pack<RT>(x[0], x[1]), w[1] = pa_pack<RT>(x[2], x[3]);
+    kv_store<8>(out + at * 2, w);
+  }
+}
+
+// Rows r0 .. r1-1 of one (sequence, key head, split) by plain sums, a key at a time: the fallback for values that are not finite.
+// buf: 3 * 256 floats of LDS.
+template <int RT, int CT>
+__device__ void pa_rows_alone(const PagedAttn& a, int b, int h, int split, int r0, int r1, const KvSpan& span, float* buf) {
+  const int tid = threadIdx.x, D = a.p.dim;
+  int* page_of = reinterpret_cast<int*>(buf);                       // -1: not seen
+  float *z_of = buf + 256, *w_of = buf + 512;
+  const int dq = min(tid, D - 1);                                   // this thread's column
+#pragma unroll 1
+  for (int r = r0; r < r1; ++r) {
+    const int t = r / a.group, hq = h * a.group + r % a.group;
+    const int lim = t >= span.fresh ? 0 : a.causal ? min(span.len - span.fresh + t + 1, span.there) : span.there;
+    const unsigned char* qr = a.q + b * a.q_seq + t * a.q_token + (long long)hq * a.q_head;
+    float top = -INFINITY, sum = 0.f, o = 0.f;
+#pragma unroll 1
+    for (long long c0 = (long long)split * a.chunk; c0 < lim; c0 += (long long)a.splits * a.chunk) {
+      const int c1 = (int)min(c0 + a.chunk, (long long)lim);
+#pragma unroll 1
+      for (int p0 = (int)c0; p0 < c1; p0 += 256) {
+        const int p = p0 + tid;
+        int page = -1;
+        if (p < c1 && (!a.padding || (p < a.padding_width && !a.padding[(long long)b * a.padding_stride + p]))) {
+          page = a.table[(long long)b * a.table_stride + (p >> a.page_shift)];
+          if ((unsigned)page >= (unsigned)a.p.num_pages) page = -1;
+        }
+        const int slot = p & (a.p.page_size - 1);
+        float z = -INFINITY;
+        if (page >= 0) {
+          const long long at = (long long)page * a.p.page_stride + (long long)h * a.p.head_stride + (long long)slot * a.p.slot_stride;
+          z = 0.f;
+          for (int d = 0; d < D; d += 8) {
+            unsigned kw[8], qw[8];
+            kv_load<kv_bytes(CT) == 4 ? 16 : kv_bytes(CT) * 8>(kw, static_cast<const unsigned char*>(a.p.k) + (at + d) * kv_bytes(CT));
+            if constexpr (kv_bytes(CT) == 4) kv_load<16>(kw + 4, static_cast<const unsigned char*>(a.p.k) + (at + d) * 4 + 16);
+            kv_load<16>(qw, qr + d * kv_bytes(RT));
+            if constexpr (kv_bytes(RT) == 4) kv_load<16>(qw + 4, qr + d * 4 + 16);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z += kv_elem<RT>(qw, i) * kv_elem<CT>(kw, i);
+          }
+          z *= a.scale_log2e;
+          if constexpr (kv_scaled(CT)) z *= a.p.k_scale[(long long)page * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + slot];
+        }
+        __syncthreads();                                            // the last block's lists have been read
+        page_of[tid] = page;
+        z_of[tid] = z;
+        __syncthreads();
+        float up = top;
+        for (int i = 0; i < 256; ++i) up = fmaxf(up, z_of[i]);
+        const float ref = up == -INFINITY ? 0.f : up;
+        const float shrink = __builtin_amdgcn_exp2f(top - ref);
+        top = up;
+        w_of[tid] = page < 0 ? 0.f : __builtin_amdgcn_exp2f(z - ref);
+        __syncthreads();
+        // (before anything was seen o and sum are 0, and shrink is 0 or 1)
+        o *= shrink, sum *= shrink;
+        for (int i = 0; i < min(256, c1 - p0); ++i) {
+          if (page_of[i] < 0) continue;
+          const int si = (p0 + i) & (a.p.page_size - 1);
+          const long long at = (long long)page_of[i] * a.p.page_stride + (long long)h * a.p.head_stride + (long long)si * a.p.slot_stride + dq;
+          const unsigned char* src = static_cast<const unsigned char*>(a.p.v) + at * kv_bytes(CT);
+          unsigned w[1];
+          if constexpr (kv_bytes(CT) == 4) w[0] = *reinterpret_cast<const unsigned*>(src);
+          else if constexpr (kv_bytes(CT) == 2) w[0] = *reinterpret_cast<const unsigned short*>(src);
+          else w[0] = *src;
+          float pv = w_of[i];
+          sum += pv;
+          if constexpr (kv_scaled(CT)) pv *= a.p.v_scale[(long long)page_of[i] * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + si];
+          o += pv * kv_elem<CT>(w, 0);
+        }
+      }
+    }
+    const long long row = ((long long)b * a.T + t) * a.q_heads + hq;
+    if (tid < D) {
+      if (a.splits > 1) {
+        a.part_o[(row * a.splits + split) * D + tid] = o;
+        if (tid == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.splits + split) * 2) = make_float2(top, sum);
+      } else {
+        const float y = sum == 0.f ? 0.f : o / sum;
+        if constexpr (RT == KV_F32) reinterpret_cast<float*>(a.out)[row * D + tid] = y;
+        else reinterpret_cast<unsigned short*>(a.out)[row * D + tid] = (unsigned short)pa_pack<RT>(y, 0.f);
+      }
+    }
+  }
+}
+
+template <int RT, int CT, int DP, int NT, bool PADDED>
+__global__ __launch_bounds__(64 * PA_WAVES) void paged_attention_kernel(const PagedAttn a) {
+  constexpr bool M16 = RT != KV_F32;
+  constexpr int QK = RT, PV = CT == KV_F16 ? KV_F16 : KV_BF16;      // operand types of the 16-bit products
+  constexpr int CB = kv_bytes(CT), RB = kv_bytes(RT);
+  constexpr int KT = M16 || DP <= 128 ? 2 : 1;                      // 16-key blocks of a tile
+  constexpr int KEYS = 16 * KT;
+  // keys: chunk i of a lane in 16-lane group g is columns i*4*KC + KC*g ...; values: column c*16*VC + VC*m + e for lane m
+  constexpr int KC = 16 / CB < DP / 4 ? 16 / CB : DP / 4, NK = DP / (4 * KC), KW = KC * CB / 4;
+  constexpr int VE = DP / 16, VC = 16 / CB < VE ? 16 / CB : VE, NV = VE / VC, VB = VC * CB, VW = (VB + 3) / 4;
+  constexpr int QN = M16 ? DP / 32 : DP / 4;                        // steps of 8 packed columns, or single columns
+  static_assert(!M16 || KC % 8 == 0, "16-bit products take 8 columns a lane");
+
+  __shared__ int s_page[PA_MAX_CHUNK / 8 + 1];
+  __shared__ __align__(16) unsigned char s_hide[PADDED ? PA_MAX_CHUNK : 16];
+  constexpr int OR = DP == 256 ? 8 : 16;                            // rows of a wave in LDS at a time
+  __shared__ __align__(16) float s_o[PA_WAVES][OR][DP + 4];
+  __shared__ float s_ml[PA_WAVES][16][2];
+
+  // which part of the work: the row groups of one (sequence, key head, split) run on one XCD and share its L2
+  unsigned unit = blockIdx.x, rg = 0;
+  if (a.row_groups > 1) {
+    const unsigned xcd = blockIdx.x & 7u, at = blockIdx.x >> 3;
+    unit = (at / a.row_groups) * 8u + xcd, rg = at % a.row_groups;
+  }
+  const unsigned heads = a.p.heads, bh = a.B * heads;
+  const int split = unit / bh;
+  if (split >= a.splits) return;
+  const int b = (unit % bh) / heads, h = unit % heads;
+  const int row0 = rg * (16 * NT);
+  const KvSpan span = kv_span(a.lens, a.new_lens, b, a.T, a.width << a.page_shift);
+  const int past = span.len - span.fresh;
+  // what the first and the last real row of this group see
+  const int t_lo = row0 / a.group, t_hi = min((min(row0 + 16 * NT, a.rows) - 1) / a.group, span.fresh - 1);
+  const int most = t_lo < span.fresh ? (a.causal ? min(past + t_hi + 1, span.there) : span.there) : 0;
+  const int least = a.causal ? min(past + t_lo + 1, span.there) : span.there;
+  const bool joined = a.splits > 1;
+  if (joined && (long long)split * a.chunk >= span.there) return;    // the join takes as many partials as there are chunks
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g = lane >> 4;
+  const int D = a.p.dim, page_mask = a.p.page_size - 1;
+
+  // query rows, in the operand layout
+  unsigned qf[NT][QN * (M16 ? 4 : 1)];
+  int lim[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = row0 + nt * 16 + m, t = r / a.group, j = r % a.group;
+    const bool real = r < a.rows && t < span.fresh;
+    lim[nt] = !real ? most : a.causal ? min(past + t + 1, span.there) : span.there;
+    const unsigned char* qr = a.q + b * a.q_seq + t * a.q_token + (long long)(h * a.group + j) * a.q_head;
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+#pragma unroll
+      for (int e = 0; e < KC; e += 16 / RB) {
+        const int d = i * 4 * KC + KC * g + e;
+        unsigned w[4] = {};
+        if (real && d < D) kv_load<16>(w, qr + d * RB);
+        const int at = (i * KC + e) * RB / 4;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) qf[nt][at + x] = w[x];
+      }
+    }
+  }
+
+  f32x4 acc[NT][VE];
+  float mrow[NT], lrow[NT];
+  const unsigned char* kbase = static_cast<const unsigned char*>(a.p.k) + (long long)h * a.p.head_stride * CB;
+  const unsigned char* vbase = static_cast<const unsigned char*>(a.p.v) + (long long)h * a.p.head_stride * CB;
+
+  {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      mrow[nt] = -INFINITY, lrow[nt] = 0.f;
+#pragma unroll
+      for (int e = 0; e < VE; ++e) acc[nt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (long long c0 = (long long)split * a.chunk; c0 < most; c0 += (long long)a.splits * a.chunk) {
+      const int c1 = (int)min(c0 + a.chunk, (long long)most);
+      const int first_page = (int)(c0 >> a.page_shift);
+      __syncthreads();                                              // the previous chunk's pages have been read
+      for (int i = tid; i <= ((c1 - 1) >> a.page_shift) - first_page; i += 64 * PA_WAVES) {
+        int page = a.table[(long long)b * a.table_stride + first_page + i];
+        if ((unsigned)page >= (unsigned)a.p.num_pages) {
+          page = -1;
+          kv_fault(a.p.faults, 4);
+        }
+        s_page[i] = page;
+      }
+      if constexpr (PADDED) {
+        for (int i = tid; i < c1 - (int)c0; i += 64 * PA_WAVES) {
+          const int p = (int)c0 + i;
+          s_hide[i] = p < a.padding_width ? a.padding[(long long)b * a.padding_stride + p] : 1;
+        }
+      }
+      __syncthreads();
+      for (int k0 = (int)c0 + wave * KEYS; k0 < c1; k0 += PA_WAVES * KEYS) {
+        // ---- loads.  Keys past the end or on a bad page read slot 0 of page 0 instead and are not seen.
+        unsigned kw[KT][NK * KW];
+#pragma unroll
+        for (int s = 0; s < KT; ++s) {
+          const int p = k0 + 16 * s + m;
+          const int page = p < c1 ? s_page[(p >> a.page_shift) - first_page] : -1;
+          const unsigned char* src = kbase + (page < 0 ? 0ll : ((long long)page * a.p.page_stride + (long long)(p & page_mask) * a.p.slot_stride) * CB);
+#pragma unroll
+          for (int i = 0; i < NK; ++i) {
+            const int d = i * 4 * KC + KC * g;
+            kv_load<KC * CB>(&kw[s][i * KW], src + (d < D ? d : 0) * CB);
+            if (d >= D) {
+#pragma unroll
+              for (int x = 0; x < KW; ++x) kw[s][i * KW + x] = 0u;
+            }
+          }
+        }
+        unsigned vw[KT * 4][NV * VW];
+        unsigned seen = 0;                                          // bit s*4+j: this lane's key 16 s + 4 g + j is there
+        float ks[KT][4], vs[KT][4];
+#pragma unroll
+        for (int s = 0; s < KT; ++s) {
+          const int p = k0 + 16 * s + 4 * g;
+          const int page = p < c1 ? s_page[(p >> a.page_shift) - first_page] : -1;
+          unsigned hide = 0;
+          if constexpr (PADDED) hide = *reinterpret_cast<const unsigned*>(&s_hide[p < c1 ? p - (int)c0 : 0]);
+          const int slot = p & page_mask;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const bool ok = page >= 0 && p + j < c1 && !((hide >> (8 * j)) & 255u);
+            seen |= (ok ? 1u : 0u) << (4 * s + j);
+            const unsigned char* src = vbase + (ok ? ((long long)page * a.p.page_stride + (long long)(slot + j) * a.p.slot_stride) * CB : 0ll);
+#pragma unroll
+            for (int c = 0; c < NV; ++c) {
+              const int d = c * 16 * VC + VC * m;
+              kv_load<VB>(&vw[4 * s + j][c * VW], src + (d < D ? d : 0) * CB);
+            }
+          }
+          if constexpr (kv_scaled(CT)) {
+            const long long at = page < 0 ? 0ll : (long long)page * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + slot;
+            kv_load<16>(reinterpret_cast<unsigned*>(ks[s]), reinterpret_cast<const unsigned char*>(a.p.k_scale + at));
+            kv_load<16>(reinterpret_cast<unsigned*>(vs[s]), reinterpret_cast<const unsigned char*>(a.p.v_scale + at));
+          }
+        }
+        const bool whole = !PADDED && k0 + KEYS <= least && __all(seen == (1u << (4 * KT)) - 1u);
+        if (!whole) {                                               // a key that nobody sees must not meet the products
+#pragma unroll
+          for (int k = 0; k < KT * 4; ++k)
+#pragma unroll
+            for (int x = 0; x < NV * VW; ++x) vw[k][x] = (seen >> k) & 1u ? vw[k][x] : 0u;
+        }
+
+        // ---- S^T = K Q^T
+        f32x4 st[NT][KT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int s = 0; s < KT; ++s) st[nt][s] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < KT; ++s) {
+          if constexpr (M16) {
+#pragma unroll
+            for (int i = 0; i < QN; ++i) {
+              unsigned kf[4];
+              if constexpr (CB == 2) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) kf[x] = kw[s][i * 4 + x];
+              } else {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) kf[x] = pa_widen<QK, CT>(kw[s][i * 2 + (x >> 1)], x & 1);
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                const unsigned qv[4] = {qf[nt][4 * i], qf[nt][4 * i + 1], qf[nt][4 * i + 2], qf[nt][4 * i + 3]};
+                st[nt][s] = pa_mfma16<QK>(kf, qv, st[nt][s]);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < QN; ++i) {
+              const float kf = kv_elem<CT>(&kw[s][(i / KC) * KW], i % KC);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                st[nt][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf, __builtin_bit_cast(float, qf[nt][i]), st[nt][s], 0, 0, 0);
+            }
+          }
+        }
+
+        // ---- softmax: base 2, scale * log2(e) folded into S
+        float pr[NT][KT * 4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float z[KT * 4], top = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < KT * 4; ++k) {
+            z[k] = st[nt][k >> 2][k & 3] * a.scale_log2e;
+            if constexpr (kv_scaled(CT)) z[k] *= ks[k >> 2][k & 3];
+            if (!whole) z[k] = ((seen >> k) & 1u) && k0 + 16 * (k >> 2) + 4 * g + (k & 3) < lim[nt] ? z[k] : -INFINITY;
+            top = fmaxf(top, z[k]);
+          }
+          top = fmaxf(pa_max4(top), mrow[nt]);
+          const float ref = top == -INFINITY ? 0.f : top;           // a row that has seen nothing yet
+          if (__any(top > mrow[nt])) {
+            const float shrink = __builtin_amdgcn_exp2f(mrow[nt] - ref);
+            lrow[nt] *= shrink;
+#pragma unroll
+            for (int e = 0; e < VE; ++e) acc[nt][e] *= shrink;
+            mrow[nt] = top;
+          }
+#pragma unroll
+          for (int k = 0; k < KT * 4; ++k) {
+            pr[nt][k] = __builtin_amdgcn_exp2f(z[k] - ref);
+            lrow[nt] += pr[nt][k];
+            if constexpr (kv_scaled(CT)) {
+              const float scaled = pr[nt][k] * vs[k >> 2][k & 3];
+              pr[nt][k] = whole || z[k] != -INFINITY ? scaled : 0.f;
+            }
+          }
+        }
+
+        // ---- O^T += V^T P^T
+        if constexpr (M16) {
+          unsigned hi[NT][4], lo[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              hi[nt][x] = pa_pack<PV>(pr[nt][2 * x], pr[nt][2 * x + 1]);
+              lo[nt][x] = pa_pack<PV>(pr[nt][2 * x] - pa_half<PV>(hi[nt][x], 0), pr[nt][2 * x + 1] - pa_half<PV>(hi[nt][x], 1));
+            }
+#pragma unroll
+          for (int c = 0; c < NV; ++c) {
+#pragma unroll
+            for (int q4 = 0; q4 < (VC + 3) / 4; ++q4) {
+              // four columns (a pair of words of 16-bit elements, a word of codes) of eight keys -> one operand per column
+              unsigned vf[4][4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                if constexpr (CB == 2) {
+#pragma unroll
+                  for (int y = 0; y < 2; ++y) {
+                    if (4 * q4 + 2 * y < VC) {
+                      const unsigned wa = vw[2 * x][c * VW + 2 * q4 + y], wb = vw[2 * x + 1][c * VW + 2 * q4 + y];
+                      vf[2 * y][x] = __builtin_amdgcn_perm(wb, wa, 0x05040100u);
+                      vf[2 * y + 1][x] = __builtin_amdgcn_perm(wb, wa, 0x07060302u);
+                    }
+                  }
+                } else {
+                  const unsigned wa = vw[2 * x][c * VW + q4], wb = vw[2 * x + 1][c * VW + q4];
+                  const unsigned t0 = __builtin_amdgcn_perm(wb, wa, 0x05010400u), t1 = __builtin_amdgcn_perm(wb, wa, 0x07030602u);
+                  vf[0][x] = pa_widen<PV, CT>(t0, false);
+                  vf[1][x] = pa_widen<PV, CT>(t0, true);
+                  if (VC > 2) {
+                    vf[2][x] = pa_widen<PV, CT>(t1, false);
+                    vf[3][x] = pa_widen<PV, CT>(t1, true);
+                  }
+                }
+              }
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                if (4 * q4 + y < VC) {
+                  const int e = c * VC + 4 * q4 + y;
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt) {
+                    acc[nt][e] = pa_mfma16<PV>(vf[y], hi[nt], acc[nt][e]);
+                    acc[nt][e] = pa_mfma16<PV>(vf[y], lo[nt], acc[nt][e]);
+                  }
+                }
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < KT * 4; ++k)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+              const float vf = kv_elem<CT>(&vw[k][(e / VC) * VW], e % VC);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) acc[nt][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, pr[nt][k], acc[nt][e], 0, 0, 0);
+            }
+        }
+      }
+    }
+  }
+
+  // What a row does not see must not reach it, but 0 * infinity and 0 * NaN do in a matrix product over shared values, and an
+  // infinite value meets the rest of its P, which may be 0 or negative.  So where a result is not finite, the rows are
+  // computed again, each from what it sees alone.
+  bool off = false;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = row0 + nt * 16 + m;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < VE; ++e)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int d = (e / VC) * 16 * VC + VC * (4 * g + j) + e % VC;
+        bad |= d < D && !(__builtin_fabsf(acc[nt][e][j]) < INFINITY);
+      }
+    off |= bad && r < a.rows && r / a.group < span.fresh;
+  }
+  if (__syncthreads_or(off)) {
+    pa_rows_alone<RT, CT>(a, b, h, split, row0, min(row0 + 16 * NT, a.rows), span, &s_o[0][0][0]);
+    return;
+  }
+
+  // ---- the four waves' parts of each row
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const float l = pa_sum4(lrow[nt]);
+#pragma unroll
+    for (int half = 0; half < 16 / OR; ++half) {
+      __syncthreads();
+      if (g == 0) s_ml[wave][m][0] = mrow[nt], s_ml[wave][m][1] = l;
+      if (m / OR == half) {
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s_o[wave][m % OR][(e / VC) * 16 * VC + VC * (4 * g + j) + e % VC] = acc[nt][e][j];
+      }
+      __syncthreads();
+      for (int i = tid; i < OR * (DP / 4); i += 64 * PA_WAVES) {
+        const int ml = i / (DP / 4) + half * OR, d = (i % (DP / 4)) * 4;
+        const int r = row0 + nt * 16 + ml, t = r / a.group;
+        if (r >= a.rows || d >= D) continue;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < PA_WAVES; ++w) top = fmaxf(top, s_ml[w][ml][0]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float sum = 0.f, o[4] = {};
+#pragma unroll
+        for (int w = 0; w < PA_WAVES; ++w) {
+          const float x = __builtin_amdgcn_exp2f(s_ml[w][ml][0] - ref);
+          sum += x * s_ml[w][ml][1];
+          const float4 v = ld4(&s_o[w][ml - half * OR][d]);
+          // a wave whose keys this row does not see adds nothing (its O is zero: no 0 * infinity comes of it)
+          o[0] += x * v.x, o[1] += x * v.y, o[2] += x * v.z, o[3] += x * v.w;
+        }
+        const long long row = ((long long)b * a.T + t) * a.q_heads + h * a.group + r % a.group;
+        if (joined) {
+          st4(a.part_o + (row * a.splits + split) * D + d, make_float4(o[0], o[1], o[2], o[3]));
+          if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.splits + split) * 2) = make_float2(top, sum);
+        } else {
+          const bool some = t < span.fresh && !(sum == 0.f);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[x] = some ? o[x] / sum : 0.f;
+          pa_store_row4<RT>(a.out, row * D + d, o);
+        }
+      }
+    }
+  }
+}
+
+template <int RT, int CT, int DP, int NT>
+static void pa_launch(const PagedAttn& a, unsigned blocks, hipStream_t stream) {
+  if (a.padding) hipLaunchKernelGGL((paged_attention_kernel<RT, CT, DP, NT, true>), dim3(blocks), dim3(64 * PA_WAVES), 0, stream, a);
+  else hipLaunchKernelGGL((paged_attention_kernel<RT, CT, DP, NT, false>), dim3(blocks), dim3(64 * PA_WAVES), 0, stream, a);
+}
+template <int RT, int CT>
+static void pa_launch(const PagedAttn& a, int tiles, unsigned blocks, hipStream_t stream) {
+  const int D = a.p.dim;
+  if (D <= 32) tiles == 2 ? pa_launch<RT, CT, 32, 2>(a, blocks, stream) : pa_launch<RT, CT, 32, 1>(a, blocks, stream);
+  else if (D <= 64) tiles == 2 ? pa_launch<RT, CT, 64, 2>(a, blocks, stream) : pa_launch<RT, CT, 64, 1>(a, blocks, stream);
+  else if (D <= 128) tiles == 2 ? pa_launch<RT, CT, 128, 2>(a, blocks, stream) : pa_launch<RT, CT, 128, 1>(a, blocks, stream);
+  else pa_launch<RT, CT, 256, 1>(a, blocks, stream);
+}
+
+// one definition per row type, each in its own source file: the instantiations compile side by side
+void pa_run_f32(const PagedAttn& a, int tiles, unsigned blocks, hipStream_t stream);
+void pa_run_bf16(const PagedAttn& a, int tiles, unsigned blocks, hipStream_t stream);
+void pa_run_f16(const PagedAttn& a, int tiles, unsigned blocks, hipStream_t stream);
+
+}  // namespace pvsg

@@ -1573,3 +1573,234 @@ def attn_mask_bits_packed(pack, feature_lowres, flags, num_queries):
 
 conv3x3s2_bf16x3_pack = conv3x3_bf16x3_pack
 conv3x3s2_bf16x3_supported = conv3x3_bf16x3_supported
+
+
+# ---- paged key/value cache (csrc/kv_cache.hip, csrc/paged_attention.h) ------------------------------------------------------
+# A live video hands over 1..32 new frames at a time.  Their keys and values are appended to pages that the video owns, and the
+# new frames' queries attend over everything cached: no frame is projected twice.  Lengths and page tables stay on the
+# device, so a step is a fixed set of launches (graph-capturable); what they may point at is checked there.
+_KV_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3, torch.int8: 4}
+_KV_ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_KV_SCALED = (torch.float8_e4m3fn, torch.int8)
+PAGED_ATTENTION_MAX_NEW = 32
+
+_page_faults = {}
+
+
+def _page_fault_word(device):
+    t = _page_faults.get(device.index)
+    if t is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError('KVPages: the first pool of a device cannot be made while a graph is captured')
+        # a blocking copy: the word is there for every stream
+        t = _page_faults[device.index] = torch.zeros(1, dtype=torch.int32).to(device)
+    return t
+
+
+def page_fault_check(device=None):
+    """Raise RuntimeError if a page table or a length sent kv_append / kv_read / paged_attention outside a pool or a table since the
+    last check, on `device` (default: the current one).  Synchronises.  What they skipped was not written, read as zeros, or
+    was not attended to."""
+    d = torch.device('cuda' if device is None else device)
+    t = _page_faults.get(d.index if d.index is not None else torch.cuda.current_device())
+    bits = int(t.item()) if t is not None else 0
+    if bits:
+        t.zero_()
+        who = [n for i, n in enumerate(('kv_append', 'kv_read', 'paged_attention')) if bits >> i & 1]
+        raise RuntimeError('%s met page ids outside the pool, or lengths past the page table: those positions were skipped'
+                           % ', '.join(who))
+
+
+class KVPages:
+    """A pool of key / value pages: k, v (num_pages, heads, page_size, head_dim), any strides with a dense last axis (a pool
+    laid out (num_pages, page_size, heads, head_dim) is passed as `.transpose(1, 2)`), float32, bfloat16, float16, or 8-bit
+    (float8_e4m3fn, int8) with a float32 scale per row, k_scale / v_scale (num_pages, heads, page_size), contiguous.
+    Slots hold x, 8-bit ones x / scale.  The pool is written in place by `kv_append`; its tensors stay the caller's."""
+
+    __slots__ = ('k', 'v', 'k_scale', 'v_scale', 'dtype', 'device', 'num_pages', 'heads', 'page_size', 'head_dim', '_struct')
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        for n, t in (('k', k), ('v', v)):
+            if not isinstance(t, torch.Tensor) or t.dim() != 4:
+                raise RuntimeError('KVPages: %s must be a (num_pages, heads, page_size, head_dim) tensor' % n)
+            if not t.is_cuda:
+                raise RuntimeError('KVPages: %s must live on a HIP device (got %s); the MI355X backend has no CPU path' % (n, t.device))
+            if t.dtype not in _KV_TYPES:
+                raise RuntimeError('KVPages: %s is %s; pools are float32, bfloat16, float16, float8_e4m3fn or int8' % (n, t.dtype))
+            if t.requires_grad:
+                raise RuntimeError('KVPages: %s requires a gradient; the pool is written in place, without autograd' % n)
+        if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.stride() != v.stride():
+            raise RuntimeError('KVPages: k and v differ in shape, strides, dtype or device')
+        P, H, S, D = k.shape
+        unit = 16 // k.element_size()
+        sp, sh, ss, sd = k.stride()
+        if P < 1 or H < 1 or S < 8 or S > 65536 or S & (S - 1):
+            raise RuntimeError('KVPages: page_size must be a power of two in [8, 65536], with at least one page and head (got %s)' % (tuple(k.shape),))
+        if D < 16 or D > 256 or D % 16:
+            raise RuntimeError('KVPages: head_dim must be a multiple of 16 up to 256 (got %d)' % D)
+        if sd != 1 or sp % unit or sh % unit or ss % unit or ss < D or (k.data_ptr() | v.data_ptr()) & 15:
+            raise RuntimeError('KVPages: rows must be dense, distinct and 16-byte aligned (strides %s)' % (k.stride(),))
+        scaled = k.dtype in _KV_SCALED
+        if scaled != (k_scale is not None) or scaled != (v_scale is not None):
+            raise RuntimeError('KVPages: k_scale and v_scale come with 8-bit pools, and only with them')
+        if scaled:
+            for n, t in (('k_scale', k_scale), ('v_scale', v_scale)):
+                if _chk(t, 'KVPages: ' + n).data_ptr() != t.data_ptr() or tuple(t.shape) != (P, H, S) or t.device != k.device or t.data_ptr() & 15:
+                    raise RuntimeError('KVPages: %s must be contiguous (num_pages, heads, page_size) on the pool\'s device' % n)
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.dtype, self.device, self.num_pages, self.heads, self.page_size, self.head_dim = k.dtype, k.device, P, H, S, D
+        self._struct = _lib.KvPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if scaled else None,
+                                    v_scale.data_ptr() if scaled else None, sp, sh, ss, H * S, S, P, H, S, D,
+                                    _KV_TYPES[k.dtype], _page_fault_word(k.device).data_ptr())
+
+    @classmethod
+    def empty(cls, num_pages, heads, page_size, head_dim, dtype=torch.float32, device='cuda'):
+        """A new pool (nothing reads a slot before it is appended to)."""
+        k, v = (torch.empty((num_pages, heads, page_size, head_dim), dtype=dtype, device=device) for _ in range(2))
+        if dtype not in _KV_SCALED:
+            return cls(k, v)
+        return cls(k, v, *(torch.empty((num_pages, heads, page_size), device=device) for _ in range(2)))
+
+
+def _kv_ints(t, name, pages, shape):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != pages.device or t.dim() != len(shape) or \
+            any(n is not None and n != m for n, m in zip(shape, t.shape)):
+        raise RuntimeError('%s must be an int32 tensor of shape %s on %s' % (name, tuple('?' if n is None else n for n in shape), pages.device))
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _kv_table(table, pages, B):
+    t = _kv_ints(table, 'table', pages, (B, None))
+    if t.shape[1] < 1 or t.shape[1] * pages.page_size > 1 << 30:
+        raise RuntimeError('table: %d pages of %d positions (one page at least, 2^30 positions at most)' % (t.shape[1], pages.page_size))
+    return t
+
+
+def _kv_aligned(t):
+    if t.stride(3) != 1 or t.data_ptr() & 15:
+        return False
+    n = 16 // t.element_size() - 1
+    return not (t.stride(0) & n or t.stride(1) & n or t.stride(2) & n)
+
+
+def _kv_rows(t, name, pages, heads):
+    """(B, T, heads, head_dim) rows of an activation type: any strides; copied where a row is not dense or not 16-byte aligned"""
+    if not isinstance(t, torch.Tensor) or t.dim() != 4:
+        raise RuntimeError('%s must be a (sequences, tokens, heads, head_dim) tensor' % name)
+    if t.device != pages.device:
+        raise RuntimeError('%s is on %s, the pool on %s' % (name, t.device, pages.device))
+    if t.dtype not in _KV_ROW_TYPES:
+        raise RuntimeError('%s must be float32, bfloat16 or float16 (got %s)' % (name, t.dtype))
+    if t.shape[3] != pages.head_dim or (t.shape[2] != heads if heads else t.shape[2] < 1 or t.shape[2] % pages.heads):
+        raise RuntimeError('%s: %d heads of %d over a pool of %d heads of %d' % (name, t.shape[2], t.shape[3], pages.heads, pages.head_dim))
+    if t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError('%s requires a gradient: the paged cache is forward only (call it under torch.no_grad())' % name)
+    if t.shape[0] > 65535:
+        raise RuntimeError('%s: %d sequences (at most 65535)' % (name, t.shape[0]))
+    if _kv_aligned(t):
+        return t
+    t = t.contiguous()
+    return t if _kv_aligned(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def kv_append(pages, k, v, table, lens, new_lens=None):
+    """Write new rows into the pool, rounding or quantising them to its type (one pass, in place).
+
+    k, v (B, T, heads, head_dim) float32 / bfloat16 / float16; table (B, W) int32: position p of sequence b is slot p % page_size of page
+    table[b, p // page_size]; lens (B,) int32: positions of each sequence INCLUDING the new ones.  Of sequence b's T rows the first
+    n = min(T, lens[b], new_lens[b]) are written, at positions lens[b] - n ..; new_lens (B,) int32 defaults to T everywhere.
+    8-bit pools: scale = max(max|row| * (1/448 or 1/127), 2^-126), code = round(row / scale), ties to even; a row with a NaN or infinity reads
+    back as NaN.  Pages that are appended to belong to one sequence.  Page ids out of the pool: skipped, see page_fault_check."""
+    k = _kv_rows(k, 'k', pages, pages.heads)
+    v = _kv_rows(v, 'v', pages, pages.heads)
+    if k.shape != v.shape or k.dtype != v.dtype:
+        raise RuntimeError('kv_append: k %s %s and v %s %s differ' % (tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
+    if k.stride() != v.stride():
+        k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
+    B, T = k.shape[:2]
+    table = _kv_table(table, pages, B)
+    lens = _kv_ints(lens, 'lens', pages, (B,))
+    new_lens = _kv_ints(new_lens, 'new_lens', pages, (B,)) if new_lens is not None else None
+    if B == 0 or T == 0:
+        return pages
+    sb, st, sh, _ = k.stride()
+    with _on(pages.device):
+        _lib.call('pvsg_kv_append', pages._struct, k.data_ptr(), v.data_ptr(), _KV_ROW_TYPES[k.dtype], sb, st, sh, table.data_ptr(),
+                  table.stride(0), table.shape[1], lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, B, T,
+                  _stream_ptr())
+    return pages
+
+
+def kv_read(pages, table, lens, length, start=0, dtype=torch.float32):
+    """Positions start .. start + length - 1 of every sequence as two dense (B, length, heads, head_dim) tensors of `dtype`
+    (float32, bfloat16, float16): code * scale, rounded once.  Rows at positions >= lens[b] are zero."""
+    if dtype not in _KV_ROW_TYPES:
+        raise RuntimeError('kv_read: dtype must be float32, bfloat16 or float16 (got %s)' % (dtype,))
+    length, start = int(length), int(start)
+    if length < 0 or start < 0 or start + length >= 1 << 31:
+        raise RuntimeError('kv_read: positions %d .. %d + %d' % (start, start, length))
+    table = _kv_table(table, pages, None)
+    B = table.shape[0]
+    if B > 65535:
+        raise RuntimeError('kv_read: %d sequences (at most 65535)' % B)
+    lens = _kv_ints(lens, 'lens', pages, (B,))
+    out = [torch.empty((B, length, pages.heads, pages.head_dim), device=pages.device, dtype=dtype) for _ in range(2)]
+    if B == 0 or length == 0:
+        return tuple(out)
+    with _on(pages.device):
+        _lib.call('pvsg_kv_read', pages._struct, out[0].data_ptr(), out[1].data_ptr(), _KV_ROW_TYPES[dtype], table.data_ptr(),
+                  table.stride(0), table.shape[1], lens.data_ptr(), B, start, length, _stream_ptr())
+    return tuple(out)
+
+
+def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None, causal=True, scale=None, max_len=None, out=None):
+    """Attention of new tokens over the cached keys and values: softmax(scale * q . k) v, in float32, rounded once to q's dtype.
+
+    q (B, T, q_heads, head_dim), T <= 32, in the pool's dtype, or float32 over any pool, or any of float32 / bfloat16 / float16 over an
+    8-bit pool; q_heads a multiple of the pool's heads (shared key heads).  table, lens, new_lens as in kv_append (append first: the new tokens
+    see themselves).  Token t of sequence b, at position lens[b] - n + t, sees the positions before lens[b]; with `causal` (default) those
+    up to its own; with key_padding_mask (B, M) bool, True = ignored as in torch's attention, and positions from M on ignored too.
+    A row that sees nothing (an empty sequence, a token past n, everything masked) is zero; what is masked never reaches a
+    result, NaN and infinities included.  scale defaults to head_dim ** -0.5.  max_len: the longest cache to plan the split for, if
+    the table holds much more (longer ones are computed all the same).  out: (B, T, q_heads, head_dim), contiguous.
+    -> (B, T, q_heads, head_dim)"""
+    q = _kv_rows(q, 'q', pages, None)
+    B, T, HQ, D = q.shape
+    if T > PAGED_ATTENTION_MAX_NEW:
+        raise RuntimeError('paged_attention: %d new tokens a sequence (at most %d: attend in pieces)' % (T, PAGED_ATTENTION_MAX_NEW))
+    if HQ // pages.heads > 1024:
+        raise RuntimeError('paged_attention: %d query heads over %d key heads' % (HQ, pages.heads))
+    if q.dtype != pages.dtype and q.dtype != torch.float32 and pages.dtype not in _KV_SCALED:
+        raise RuntimeError('paged_attention: %s rows over a %s pool' % (q.dtype, pages.dtype))
+    table = _kv_table(table, pages, B)
+    lens = _kv_ints(lens, 'lens', pages, (B,))
+    new_lens = _kv_ints(new_lens, 'new_lens', pages, (B,)) if new_lens is not None else None
+    mask, ms, mw = None, 0, 0
+    if key_padding_mask is not None:
+        mask = key_padding_mask
+        if not isinstance(mask, torch.Tensor) or mask.dtype != torch.bool or mask.device != pages.device or mask.dim() != 2 or mask.shape[0] != B:
+            raise RuntimeError('paged_attention: key_padding_mask must be a (%d, positions) bool tensor on %s' % (B, pages.device))
+        if mask.shape[1] and mask.stride(1) != 1:
+            mask = mask.contiguous()
+        ms, mw = mask.stride(0), mask.shape[1]
+    if out is None:
+        out = torch.empty((B, T, HQ, D), device=q.device, dtype=q.dtype)
+    elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or \
+            out.data_ptr() & 15 or out.requires_grad:
+        raise RuntimeError('paged_attention: out must be a contiguous, 16-byte aligned %s tensor of shape %s on %s' % (q.dtype, tuple(q.shape), q.device))
+    if mask is not None and mw == 0:
+        return out.zero_()
+    if B == 0 or T == 0:
+        return out
+    longest = table.shape[1] * pages.page_size
+    if max_len is not None:
+        longest = max(1, min(longest, int(max_len)))
+    splits = _lib.load().pvsg_paged_attention_splits(B, T, HQ, pages.heads, D, _KV_TYPES[pages.dtype], longest)
+    work = torch.empty((B * T * HQ * splits * (D + 2),), device=q.device, dtype=torch.float32) if splits > 1 else None
+    sb, st, sh, _ = q.stride()
+    with _on(pages.device):
+        _lib.call('pvsg_paged_attention', pages._struct, q.data_ptr(), sb, st, sh, out.data_ptr(), _KV_ROW_TYPES[q.dtype], table.data_ptr(),
+                  table.stride(0), table.shape[1], lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None,
+                  mask.data_ptr() if mask is not None else None, ms, mw, B, T, HQ, D ** -0.5 if scale is None else float(scale),
+                  1 if causal else 0, longest, splits, work.data_ptr() if work is not None else None, _stream_ptr())
+    return out
