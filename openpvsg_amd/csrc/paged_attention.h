@@ -178,11 +178,11 @@ __device__ void pa_rows_alone(const PagedAttn& a, int b, int h, int split, int r
 }
 
 template <int RT, int CT, int DP, int NT, bool PADDED>
-__global__ __launch_bounds__(64 * PA_WAVES) void paged_attention_kernel(const PagedAttn a) {
+__global__ __launch_bounds__(64 * PA_WAVES, DP <= 128 ? 2 : 1) void paged_attention_kernel(const PagedAttn a) {
   constexpr bool M16 = RT != KV_F32;
   constexpr int QK = RT, PV = CT == KV_F16 ? KV_F16 : KV_BF16;      // operand types of the 16-bit products
   constexpr int CB = kv_bytes(CT), RB = kv_bytes(RT);
-  constexpr int KT = M16 || DP <= 128 ? 2 : 1;                      // 16-key blocks of a tile
+  constexpr int KT = M16 || DP <= 32 ? 2 : 1;                       // 16-key blocks of a tile
   constexpr int KEYS = 16 * KT;
   // keys: chunk i of a lane in 16-lane group g is columns i*4*KC + KC*g ...; values: column c*16*VC + VC*m + e for lane m
   constexpr int KC = 16 / CB < DP / 4 ? 16 / CB : DP / 4, NK = DP / (4 * KC), KW = KC * CB / 4;
