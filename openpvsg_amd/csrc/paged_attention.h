@@ -12,9 +12,13 @@
 //
 // Rounding: 16-bit rows multiply in their own type, exact products in f32 sums; 8-bit codes convert to it exactly and their
 // scales multiply S and P in f32.  P goes to the matrix cores as a 16-bit high part plus a 16-bit rest (one part alone adds an error as
-// large as the rounding of the result itself).  f32 rows run in f32 throughout.
+// large as the rounding of the result itself).  f32 rows over a bf16 or 8-bit pool go as three bf16 parts, which hold all
+// 24 bits, and so does their P: three 16-bit products take an eighth of the matrix cores' time that the f32 ones would.  f32 rows over a
+// f32 or f16 pool run on the f32 products.
 #pragma once
 #include "kv_pages.h"
+
+#include <type_traits>
 
 namespace pvsg {
 
@@ -71,8 +75,15 @@ __device__ __forceinline__ unsigned pa_widen(unsigned w, bool hi) {
 
 // maximum / sum over the four 16-lane groups of a wave, in every lane
 __device__ __forceinline__ float pa_max4(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  // swapping 16-lane rows of x with itself leaves rows 0 0 2 2 of x in one result and 1 1 3 3 in the other; then halves alike
+  unsigned u = __builtin_bit_cast(unsigned, x);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const unsigned r0 = r[0], r1 = r[1];
+  x = fmaxf(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+  u = __builtin_bit_cast(unsigned, x);
+  const auto q = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const unsigned q0 = q[0], q1 = q[1];
+  return fmaxf(__builtin_bit_cast(float, q0), __builtin_bit_cast(float, q1));
 }
 __device__ __forceinline__ float pa_sum4(float x) {
   x += __shfl_xor(x, 16);
@@ -177,10 +188,21 @@ __device__ void pa_rows_alone(const PagedAttn& a, int b, int h, int split, int r
   }
 }
 
+// 16-bit parts that a f32 value is multiplied in: 3 of bf16 hold all its 24 bits
+template <int PARTS, int MT>
+__device__ __forceinline__ void pa_parts(float a, float b, unsigned (&w)[PARTS]) {
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    w[i] = pa_pack<MT>(a, b);
+    a -= pa_half<MT>(w[i], 0), b -= pa_half<MT>(w[i], 1);
+  }
+}
+
 template <int RT, int CT, int DP, int NT, bool PADDED>
 __global__ __launch_bounds__(64 * PA_WAVES, DP <= 128 ? 2 : 1) void paged_attention_kernel(const PagedAttn a) {
-  constexpr bool M16 = RT != KV_F32;
-  constexpr int QK = RT, PV = CT == KV_F16 ? KV_F16 : KV_BF16;      // operand types of the 16-bit products
+  constexpr bool M16 = RT != KV_F32 || CT == KV_BF16 || kv_scaled(CT);
+  constexpr int QK = RT == KV_F16 ? KV_F16 : KV_BF16, PV = CT == KV_F16 ? KV_F16 : KV_BF16;      // operand types of the 16-bit products
+  constexpr int QL = RT == KV_F32 ? 3 : 1, PL = RT == KV_F32 ? 3 : 2;
   constexpr int CB = kv_bytes(CT), RB = kv_bytes(RT);
   constexpr int KT = M16 || DP <= 32 ? 2 : 1;                       // 16-key blocks of a tile
   constexpr int KEYS = 16 * KT;
@@ -220,7 +242,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, DP <= 128 ? 2 : 1) void paged_attent
   const int D = a.p.dim, page_mask = a.p.page_size - 1;
 
   // query rows, in the operand layout
-  unsigned qf[NT][QN * (M16 ? 4 : 1)];
+  unsigned qf[NT][QN * (M16 ? 4 * QL : 1)];
   int lim[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -228,234 +250,269 @@ __global__ __launch_bounds__(64 * PA_WAVES, DP <= 128 ? 2 : 1) void paged_attent
     const bool real = r < a.rows && t < span.fresh;
     lim[nt] = !real ? most : a.causal ? min(past + t + 1, span.there) : span.there;
     const unsigned char* qr = a.q + b * a.q_seq + t * a.q_token + (long long)(h * a.group + j) * a.q_head;
+    constexpr int STEP = M16 ? 8 : 4;
 #pragma unroll
-    for (int i = 0; i < NK; ++i) {
+    for (int i = 0; i < DP / 4 / STEP; ++i) {
+      const int d = (i * STEP / KC) * 4 * KC + KC * g + i * STEP % KC;
+      unsigned w[STEP * RB / 4] = {};
+      if (real && d < D) {
+        kv_load<16>(w, qr + d * RB);
+        if constexpr (STEP * RB == 32) kv_load<16>(w + 4, qr + d * RB + 16);
+      }
 #pragma unroll
-      for (int e = 0; e < KC; e += 16 / RB) {
-        const int d = i * 4 * KC + KC * g + e;
-        unsigned w[4] = {};
-        if (real && d < D) kv_load<16>(w, qr + d * RB);
-        const int at = (i * KC + e) * RB / 4;
+      for (int x = 0; x < 4; ++x) {
+        if constexpr (M16 && QL > 1) {
+          unsigned part[QL];
+          pa_parts<QL, QK>(kv_elem<RT>(w, 2 * x), kv_elem<RT>(w, 2 * x + 1), part);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) qf[nt][at + x] = w[x];
+          for (int l = 0; l < QL; ++l) qf[nt][(i * QL + l) * 4 + x] = part[l];
+        } else {
+          qf[nt][i * 4 + x] = w[x];
+        }
       }
     }
   }
 
   f32x4 acc[NT][VE];
   float mrow[NT], lrow[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    mrow[nt] = -INFINITY, lrow[nt] = 0.f;
+#pragma unroll
+    for (int e = 0; e < VE; ++e) acc[nt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   const unsigned char* kbase = static_cast<const unsigned char*>(a.p.k) + (long long)h * a.p.head_stride * CB;
   const unsigned char* vbase = static_cast<const unsigned char*>(a.p.v) + (long long)h * a.p.head_stride * CB;
 
-  {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      mrow[nt] = -INFINITY, lrow[nt] = 0.f;
-#pragma unroll
-      for (int e = 0; e < VE; ++e) acc[nt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // A tile's keys are loaded while the tile before is still in its softmax and its second product, its values while its own
+  // first product runs: each goes to the registers that the tile before has just done with, so nothing is held twice.
+  unsigned kw[KT][NK * KW], vw[KT * 4][NV * VW];
+  unsigned seen = 0;                                                // bit s*4+j: this lane's key 16 s + 4 g + j is there
+  float ks[KT][4], vs[KT][4];
+
+  for (long long c0 = (long long)split * a.chunk; c0 < most; c0 += (long long)a.splits * a.chunk) {
+    const int c1 = (int)min(c0 + a.chunk, (long long)most);
+    const int first_page = (int)(c0 >> a.page_shift);
+    __syncthreads();                                                // the previous chunk's pages have been read
+    for (int i = tid; i <= ((c1 - 1) >> a.page_shift) - first_page; i += 64 * PA_WAVES) {
+      int page = a.table[(long long)b * a.table_stride + first_page + i];
+      if ((unsigned)page >= (unsigned)a.p.num_pages) {
+        page = -1;
+        kv_fault(a.p.faults, 4);
+      }
+      s_page[i] = page;
     }
-    for (long long c0 = (long long)split * a.chunk; c0 < most; c0 += (long long)a.splits * a.chunk) {
-      const int c1 = (int)min(c0 + a.chunk, (long long)most);
-      const int first_page = (int)(c0 >> a.page_shift);
-      __syncthreads();                                              // the previous chunk's pages have been read
-      for (int i = tid; i <= ((c1 - 1) >> a.page_shift) - first_page; i += 64 * PA_WAVES) {
-        int page = a.table[(long long)b * a.table_stride + first_page + i];
-        if ((unsigned)page >= (unsigned)a.p.num_pages) {
-          page = -1;
-          kv_fault(a.p.faults, 4);
-        }
-        s_page[i] = page;
+    if constexpr (PADDED) {
+      for (int i = tid; i < c1 - (int)c0; i += 64 * PA_WAVES) {
+        const int p = (int)c0 + i;
+        s_hide[i] = p < a.padding_width && !a.padding[(long long)b * a.padding_stride + p] ? 0 : 1;
       }
-      if constexpr (PADDED) {
-        for (int i = tid; i < c1 - (int)c0; i += 64 * PA_WAVES) {
-          const int p = (int)c0 + i;
-          s_hide[i] = p < a.padding_width ? a.padding[(long long)b * a.padding_stride + p] : 1;
+    }
+    __syncthreads();
+
+    // Keys past the end read their slot of the last page (in the pool, whatever it holds), keys of a bad page that of page 0;
+    // neither is seen.
+    auto load_k = [&](int k0) {
+#pragma unroll
+      for (int s = 0; s < KT; ++s) {
+        const int p = k0 + 16 * s + m;
+        const int page = max(s_page[(min(p, c1 - 1) >> a.page_shift) - first_page], 0);
+        const unsigned char* src = kbase + ((long long)page * a.p.page_stride + (long long)(p & page_mask) * a.p.slot_stride) * CB;
+#pragma unroll
+        for (int i = 0; i < NK; ++i) {
+          const int d = i * 4 * KC + KC * g;
+          kv_load<KC * CB>(&kw[s][i * KW], src + (d < D ? d : 0) * CB);
         }
       }
-      __syncthreads();
-      for (int k0 = (int)c0 + wave * KEYS; k0 < c1; k0 += PA_WAVES * KEYS) {
-        // ---- loads.  Keys past the end or on a bad page read slot 0 of page 0 instead and are not seen.
-        unsigned kw[KT][NK * KW];
+    };
+    auto load_v = [&](int k0) {
+      seen = 0;
 #pragma unroll
-        for (int s = 0; s < KT; ++s) {
-          const int p = k0 + 16 * s + m;
-          const int page = p < c1 ? s_page[(p >> a.page_shift) - first_page] : -1;
-          const unsigned char* src = kbase + (page < 0 ? 0ll : ((long long)page * a.p.page_stride + (long long)(p & page_mask) * a.p.slot_stride) * CB);
-#pragma unroll
-          for (int i = 0; i < NK; ++i) {
-            const int d = i * 4 * KC + KC * g;
-            kv_load<KC * CB>(&kw[s][i * KW], src + (d < D ? d : 0) * CB);
-            if (d >= D) {
-#pragma unroll
-              for (int x = 0; x < KW; ++x) kw[s][i * KW + x] = 0u;
-            }
-          }
+      for (int s = 0; s < KT; ++s) {
+        const int p = k0 + 16 * s + 4 * g;                          // four keys of one page
+        const int page = s_page[(min(p, c1 - 1) >> a.page_shift) - first_page], slot = p & page_mask;
+        unsigned there = page >= 0 ? (1u << min(max(c1 - p, 0), 4)) - 1u : 0u;
+        if constexpr (PADDED) {
+          const unsigned x = ~*reinterpret_cast<const unsigned*>(&s_hide[p < c1 ? p - (int)c0 : 0]);
+          there &= (x & 1u) | (x >> 7 & 2u) | (x >> 14 & 4u) | (x >> 21 & 8u);
         }
-        unsigned vw[KT * 4][NV * VW];
-        unsigned seen = 0;                                          // bit s*4+j: this lane's key 16 s + 4 g + j is there
-        float ks[KT][4], vs[KT][4];
+        seen |= there << (4 * s);
+        const unsigned char* src = vbase + ((long long)max(page, 0) * a.p.page_stride + (long long)slot * a.p.slot_stride) * CB;
 #pragma unroll
-        for (int s = 0; s < KT; ++s) {
-          const int p = k0 + 16 * s + 4 * g;
-          const int page = p < c1 ? s_page[(p >> a.page_shift) - first_page] : -1;
-          unsigned hide = 0;
-          if constexpr (PADDED) hide = *reinterpret_cast<const unsigned*>(&s_hide[p < c1 ? p - (int)c0 : 0]);
-          const int slot = p & page_mask;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const bool ok = page >= 0 && p + j < c1 && !((hide >> (8 * j)) & 255u);
-            seen |= (ok ? 1u : 0u) << (4 * s + j);
-            const unsigned char* src = vbase + (ok ? ((long long)page * a.p.page_stride + (long long)(slot + j) * a.p.slot_stride) * CB : 0ll);
-#pragma unroll
-            for (int c = 0; c < NV; ++c) {
-              const int d = c * 16 * VC + VC * m;
-              kv_load<VB>(&vw[4 * s + j][c * VW], src + (d < D ? d : 0) * CB);
-            }
-          }
-          if constexpr (kv_scaled(CT)) {
-            const long long at = page < 0 ? 0ll : (long long)page * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + slot;
-            kv_load<16>(reinterpret_cast<unsigned*>(ks[s]), reinterpret_cast<const unsigned char*>(a.p.k_scale + at));
-            kv_load<16>(reinterpret_cast<unsigned*>(vs[s]), reinterpret_cast<const unsigned char*>(a.p.v_scale + at));
-          }
-        }
-        const bool whole = !PADDED && k0 + KEYS <= least && __all(seen == (1u << (4 * KT)) - 1u);
-        if (!whole) {                                               // a key that nobody sees must not meet the products
-#pragma unroll
-          for (int k = 0; k < KT * 4; ++k)
-#pragma unroll
-            for (int x = 0; x < NV * VW; ++x) vw[k][x] = (seen >> k) & 1u ? vw[k][x] : 0u;
-        }
-
-        // ---- S^T = K Q^T
-        f32x4 st[NT][KT];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int s = 0; s < KT; ++s) st[nt][s] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < KT; ++s) {
-          if constexpr (M16) {
-#pragma unroll
-            for (int i = 0; i < QN; ++i) {
-              unsigned kf[4];
-              if constexpr (CB == 2) {
-#pragma unroll
-                for (int x = 0; x < 4; ++x) kf[x] = kw[s][i * 4 + x];
-              } else {
-#pragma unroll
-                for (int x = 0; x < 4; ++x) kf[x] = pa_widen<QK, CT>(kw[s][i * 2 + (x >> 1)], x & 1);
-              }
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                const unsigned qv[4] = {qf[nt][4 * i], qf[nt][4 * i + 1], qf[nt][4 * i + 2], qf[nt][4 * i + 3]};
-                st[nt][s] = pa_mfma16<QK>(kf, qv, st[nt][s]);
-              }
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < QN; ++i) {
-              const float kf = kv_elem<CT>(&kw[s][(i / KC) * KW], i % KC);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                st[nt][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf, __builtin_bit_cast(float, qf[nt][i]), st[nt][s], 0, 0, 0);
-            }
-          }
-        }
-
-        // ---- softmax: base 2, scale * log2(e) folded into S
-        float pr[NT][KT * 4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float z[KT * 4], top = -INFINITY;
-#pragma unroll
-          for (int k = 0; k < KT * 4; ++k) {
-            z[k] = st[nt][k >> 2][k & 3] * a.scale_log2e;
-            if constexpr (kv_scaled(CT)) z[k] *= ks[k >> 2][k & 3];
-            if (!whole) z[k] = ((seen >> k) & 1u) && k0 + 16 * (k >> 2) + 4 * g + (k & 3) < lim[nt] ? z[k] : -INFINITY;
-            top = fmaxf(top, z[k]);
-          }
-          top = fmaxf(pa_max4(top), mrow[nt]);
-          const float ref = top == -INFINITY ? 0.f : top;           // a row that has seen nothing yet
-          if (__any(top > mrow[nt])) {
-            const float shrink = __builtin_amdgcn_exp2f(mrow[nt] - ref);
-            lrow[nt] *= shrink;
-#pragma unroll
-            for (int e = 0; e < VE; ++e) acc[nt][e] *= shrink;
-            mrow[nt] = top;
-          }
-#pragma unroll
-          for (int k = 0; k < KT * 4; ++k) {
-            pr[nt][k] = __builtin_amdgcn_exp2f(z[k] - ref);
-            lrow[nt] += pr[nt][k];
-            if constexpr (kv_scaled(CT)) {
-              const float scaled = pr[nt][k] * vs[k >> 2][k & 3];
-              pr[nt][k] = whole || z[k] != -INFINITY ? scaled : 0.f;
-            }
-          }
-        }
-
-        // ---- O^T += V^T P^T
-        if constexpr (M16) {
-          unsigned hi[NT][4], lo[NT][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              hi[nt][x] = pa_pack<PV>(pr[nt][2 * x], pr[nt][2 * x + 1]);
-              lo[nt][x] = pa_pack<PV>(pr[nt][2 * x] - pa_half<PV>(hi[nt][x], 0), pr[nt][2 * x + 1] - pa_half<PV>(hi[nt][x], 1));
-            }
+        for (int j = 0; j < 4; ++j) {
 #pragma unroll
           for (int c = 0; c < NV; ++c) {
+            const int d = c * 16 * VC + VC * m;
+            kv_load<VB>(&vw[4 * s + j][c * VW], src + (long long)j * a.p.slot_stride * CB + (d < D ? d : 0) * CB);
+          }
+        }
+        if constexpr (kv_scaled(CT)) {
+          const long long at = (long long)max(page, 0) * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + slot;
+          kv_load<16>(reinterpret_cast<unsigned*>(ks[s]), reinterpret_cast<const unsigned char*>(a.p.k_scale + at));
+          kv_load<16>(reinterpret_cast<unsigned*>(vs[s]), reinterpret_cast<const unsigned char*>(a.p.v_scale + at));
+        }
+      }
+    };
+
+    // One tile, and the loads of the wave's next one where there is one: that is known to the compiler, since a wait for the
+    // values in flight must not depend on a branch over the loads behind them.  (Columns of K past the row's end hold other columns
+    // of it and meet zeros of Q; if those are not finite, neither is the result, see below.)
+    auto tile = [&](int k0, auto more) {
+      // ---- S^T = K Q^T
+      f32x4 st[NT][KT];
 #pragma unroll
-            for (int q4 = 0; q4 < (VC + 3) / 4; ++q4) {
-              // four columns (a pair of words of 16-bit elements, a word of codes) of eight keys -> one operand per column
-              unsigned vf[4][4];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                if constexpr (CB == 2) {
+        for (int s = 0; s < KT; ++s) st[nt][s] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                  for (int y = 0; y < 2; ++y) {
-                    if (4 * q4 + 2 * y < VC) {
-                      const unsigned wa = vw[2 * x][c * VW + 2 * q4 + y], wb = vw[2 * x + 1][c * VW + 2 * q4 + y];
-                      vf[2 * y][x] = __builtin_amdgcn_perm(wb, wa, 0x05040100u);
-                      vf[2 * y + 1][x] = __builtin_amdgcn_perm(wb, wa, 0x07060302u);
-                    }
-                  }
-                } else {
-                  const unsigned wa = vw[2 * x][c * VW + q4], wb = vw[2 * x + 1][c * VW + q4];
-                  const unsigned t0 = __builtin_amdgcn_perm(wb, wa, 0x05010400u), t1 = __builtin_amdgcn_perm(wb, wa, 0x07030602u);
-                  vf[0][x] = pa_widen<PV, CT>(t0, false);
-                  vf[1][x] = pa_widen<PV, CT>(t0, true);
-                  if (VC > 2) {
-                    vf[2][x] = pa_widen<PV, CT>(t1, false);
-                    vf[3][x] = pa_widen<PV, CT>(t1, true);
-                  }
-                }
+      for (int s = 0; s < KT; ++s) {
+        if constexpr (M16) {
+#pragma unroll
+          for (int i = 0; i < QN; ++i) {
+            unsigned kf[4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) kf[x] = CB == 2 ? kw[s][i * 4 + x] : pa_widen<QK, CT>(kw[s][(i * 4 + x) / 2], x & 1);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int l = 0; l < QL; ++l) {
+                const unsigned* qp = &qf[nt][(i * QL + l) * 4];
+                const unsigned qv[4] = {qp[0], qp[1], qp[2], qp[3]};
+                st[nt][s] = pa_mfma16<QK>(kf, qv, st[nt][s]);
               }
-#pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                if (4 * q4 + y < VC) {
-                  const int e = c * VC + 4 * q4 + y;
-#pragma unroll
-                  for (int nt = 0; nt < NT; ++nt) {
-                    acc[nt][e] = pa_mfma16<PV>(vf[y], hi[nt], acc[nt][e]);
-                    acc[nt][e] = pa_mfma16<PV>(vf[y], lo[nt], acc[nt][e]);
-                  }
-                }
-              }
-            }
           }
         } else {
 #pragma unroll
-          for (int k = 0; k < KT * 4; ++k)
+          for (int i = 0; i < QN; ++i) {
+            const float kf = kv_elem<CT>(&kw[s][(i / KC) * KW], i % KC);
 #pragma unroll
-            for (int e = 0; e < VE; ++e) {
-              const float vf = kv_elem<CT>(&vw[k][(e / VC) * VW], e % VC);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) acc[nt][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, pr[nt][k], acc[nt][e], 0, 0, 0);
-            }
+            for (int nt = 0; nt < NT; ++nt)
+              st[nt][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf, __builtin_bit_cast(float, qf[nt][i]), st[nt][s], 0, 0, 0);
+          }
         }
       }
+      if constexpr (more.value) load_k(k0 + PA_WAVES * KEYS);
+
+      // ---- softmax: base 2, scale * log2(e) folded into S
+      const bool whole = !PADDED && k0 + KEYS <= least && __all(seen == (1u << (4 * KT)) - 1u);
+      float pr[NT][KT * 4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float z[KT * 4], top = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < KT * 4; ++k) {
+          z[k] = st[nt][k >> 2][k & 3] * a.scale_log2e;
+          if constexpr (kv_scaled(CT)) z[k] *= ks[k >> 2][k & 3];
+        }
+        if (!whole) {
+#pragma unroll
+          for (int k = 0; k < KT * 4; ++k) z[k] = ((seen >> k) & 1u) && k0 + 16 * (k >> 2) + 4 * g + (k & 3) < lim[nt] ? z[k] : -INFINITY;
+        }
+#pragma unroll
+        for (int k = 0; k < KT * 4; ++k) top = fmaxf(top, z[k]);
+        top = fmaxf(pa_max4(top), mrow[nt]);
+        const float ref = top == -INFINITY ? 0.f : top;             // a row that has seen nothing yet
+        if (__any(top > mrow[nt])) {
+          const float shrink = __builtin_amdgcn_exp2f(mrow[nt] - ref);
+          lrow[nt] *= shrink;
+#pragma unroll
+          for (int e = 0; e < VE; ++e) acc[nt][e] *= shrink;
+          mrow[nt] = top;
+        }
+#pragma unroll
+        for (int k = 0; k < KT * 4; ++k) {
+          pr[nt][k] = __builtin_amdgcn_exp2f(z[k] - ref);
+          lrow[nt] += pr[nt][k];
+        }
+        if constexpr (kv_scaled(CT)) {
+#pragma unroll
+          for (int k = 0; k < KT * 4; ++k) pr[nt][k] *= vs[k >> 2][k & 3];
+          if (!whole) {
+#pragma unroll
+            for (int k = 0; k < KT * 4; ++k) pr[nt][k] = z[k] != -INFINITY ? pr[nt][k] : 0.f;
+          }
+        }
+      }
+      if (!whole) {                                                 // a key that nobody sees must not meet the products
+#pragma unroll
+        for (int k = 0; k < KT * 4; ++k)
+#pragma unroll
+          for (int x = 0; x < NV * VW; ++x) vw[k][x] = (seen >> k) & 1u ? vw[k][x] : 0u;
+      }
+
+      // ---- O^T += V^T P^T
+      if constexpr (M16) {
+        unsigned pf[NT][PL][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            unsigned part[PL];
+            pa_parts<PL, PV>(pr[nt][2 * x], pr[nt][2 * x + 1], part);
+#pragma unroll
+            for (int l = 0; l < PL; ++l) pf[nt][l][x] = part[l];
+          }
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+#pragma unroll
+          for (int q4 = 0; q4 < (VC + 3) / 4; ++q4) {
+            // four columns (a pair of words of 16-bit elements, a word of codes) of eight keys -> one operand per column
+            unsigned vf[4][4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              if constexpr (CB == 2) {
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                  if (4 * q4 + 2 * y < VC) {
+                    const unsigned wa = vw[2 * x][c * VW + 2 * q4 + y], wb = vw[2 * x + 1][c * VW + 2 * q4 + y];
+                    vf[2 * y][x] = __builtin_amdgcn_perm(wb, wa, 0x05040100u);
+                    vf[2 * y + 1][x] = __builtin_amdgcn_perm(wb, wa, 0x07060302u);
+                  }
+                }
+              } else {
+                const unsigned wa = vw[2 * x][c * VW + q4], wb = vw[2 * x + 1][c * VW + q4];
+                const unsigned t0 = __builtin_amdgcn_perm(wb, wa, 0x05010400u), t1 = __builtin_amdgcn_perm(wb, wa, 0x07030602u);
+                vf[0][x] = pa_widen<PV, CT>(t0, false);
+                vf[1][x] = pa_widen<PV, CT>(t0, true);
+                if (VC > 2) {
+                  vf[2][x] = pa_widen<PV, CT>(t1, false);
+                  vf[3][x] = pa_widen<PV, CT>(t1, true);
+                }
+              }
+            }
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              if (4 * q4 + y < VC) {
+                const int e = c * VC + 4 * q4 + y;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int l = 0; l < PL; ++l) acc[nt][e] = pa_mfma16<PV>(vf[y], pf[nt][l], acc[nt][e]);
+              }
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < KT * 4; ++k)
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const float vf = kv_elem<CT>(&vw[k][(e / VC) * VW], e % VC);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) acc[nt][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, pr[nt][k], acc[nt][e], 0, 0, 0);
+          }
+      }
+      if constexpr (more.value) load_v(k0 + PA_WAVES * KEYS);
+    };
+
+    int k0 = (int)c0 + wave * KEYS;
+    if (k0 < c1) {
+      load_k(k0);
+      __builtin_amdgcn_sched_barrier(0);                            // keys first: the values are waited for later
+      load_v(k0);
+#pragma unroll 1
+      for (; k0 + PA_WAVES * KEYS < c1; k0 += PA_WAVES * KEYS) tile(k0, std::true_type{});
+      tile(k0, std::false_type{});
     }
   }
 
@@ -538,8 +595,9 @@ static void pa_launch(const PagedAttn& a, int tiles, unsigned blocks, hipStream_
   const int D = a.p.dim;
   if (D <= 32) tiles == 2 ? pa_launch<RT, CT, 32, 2>(a, blocks, stream) : pa_launch<RT, CT, 32, 1>(a, blocks, stream);
   else if (D <= 64) tiles == 2 ? pa_launch<RT, CT, 64, 2>(a, blocks, stream) : pa_launch<RT, CT, 64, 1>(a, blocks, stream);
-  else if (D <= 128) tiles == 2 ? pa_launch<RT, CT, 128, 2>(a, blocks, stream) : pa_launch<RT, CT, 128, 1>(a, blocks, stream);
-  else pa_launch<RT, CT, 256, 1>(a, blocks, stream);
+  else if (D > 128) pa_launch<RT, CT, 256, 1>(a, blocks, stream);
+  else if constexpr (RT == KV_F32) pa_launch<RT, CT, 128, 1>(a, blocks, stream);
+  else tiles == 2 ? pa_launch<RT, CT, 128, 2>(a, blocks, stream) : pa_launch<RT, CT, 128, 1>(a, blocks, stream);
 }
 
 // one definition per row type, each in its own source file: the instantiations compile side by side

@@ -47,15 +47,14 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
 }
 
 // 16-row tiles a wave carries: two where there are more rows than one tile holds and the accumulators of two fit
-static int pa_tiles(int rows, int dim) { return rows > 16 && dim <= 128 ? 2 : 1; }
+static int pa_tiles(int rows, int dim, int row_type) { return rows > 16 && dim <= (row_type == KV_F32 ? 64 : 128) ? 2 : 1; }
 
 }  // namespace pvsg
 
-extern "C" int pvsg_paged_attention_splits(int B, int T, int q_heads, int kv_heads, int dim, int type, long long max_len) {
+extern "C" int pvsg_paged_attention_splits(int B, int T, int q_heads, int kv_heads, int dim, int row_type, long long max_len) {
   using namespace pvsg;
   if (B <= 0 || T <= 0 || kv_heads <= 0 || q_heads < kv_heads || max_len <= 0) return 1;
-  (void)type;
-  const int rows = T * (q_heads / kv_heads), per = 16 * pa_tiles(rows, dim);
+  const int rows = T * (q_heads / kv_heads), per = 16 * pa_tiles(rows, dim, row_type);
   const long long units = (long long)B * kv_heads * ((rows + per - 1) / per);
   const long long tiles = (max_len + 127) / 128;                    // one 32-key tile for each wave
   long long n = (2048 + units - 1) / units;
@@ -89,7 +88,7 @@ extern "C" int pvsg_paged_attention(const pvsg_kv_pages* pages, const void* q, l
   a.width = table_width, a.padding_width = padding_width;
   while ((1 << a.page_shift) < pages->page_size) ++a.page_shift;
   a.B = B, a.T = T, a.q_heads = q_heads, a.group = q_heads / pages->heads, a.rows = T * a.group, a.splits = splits, a.causal = causal;
-  const int tiles = pa_tiles(a.rows, pages->dim);
+  const int tiles = pa_tiles(a.rows, pages->dim, row_type);
   a.row_groups = (a.rows + 16 * tiles - 1) / (16 * tiles);
   const long long capacity = (long long)table_width * pages->page_size;
   const long long longest = max_len > 0 && max_len < capacity ? max_len : capacity;

@@ -1795,7 +1795,7 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
     longest = table.shape[1] * pages.page_size
     if max_len is not None:
         longest = max(1, min(longest, int(max_len)))
-    splits = _lib.load().pvsg_paged_attention_splits(B, T, HQ, pages.heads, D, _KV_TYPES[pages.dtype], longest)
+    splits = _lib.load().pvsg_paged_attention_splits(B, T, HQ, pages.heads, D, _KV_ROW_TYPES[q.dtype], longest)
     work = torch.empty((B * T * HQ * splits * (D + 2),), device=q.device, dtype=torch.float32) if splits > 1 else None
     sb, st, sh, _ = q.stride()
     with _on(pages.device):
