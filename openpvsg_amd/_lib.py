@@ -152,16 +152,16 @@ SIGNATURES = {
     'pvsg_conv3x3s2_affine': [_c_f] * 5 + [_i] * 6 + [_c_f],
     'pvsg_kv_append': [ctypes.POINTER(KvPages), _c_f, _c_f, _i, _ll, _ll, _ll, _c_f, _ll, _i, _c_f, _c_f, _i, _i, _c_f],
     'pvsg_kv_read': [ctypes.POINTER(KvPages), _c_f, _c_f, _i, _c_f, _ll, _i, _c_f, _i, _i, _i, _c_f],
-    'pvsg_paged_attention_splits': [_i] * 6 + [_ll],
+    'pvsg_paged_attention_workspace_bytes': [ctypes.POINTER(KvPages), _i, _i, _i, _i, _i, _ll],
     'pvsg_paged_attention': [ctypes.POINTER(KvPages), _c_f, _ll, _ll, _ll, _c_f, _i, _c_f, _ll, _i, _c_f, _c_f, _c_f, _ll, _i, _i, _i,
-                             _i, _f, _i, _ll, _i, _c_f, _c_f],
+                             _i, _f, _i, _ll, _c_f, _c_f],
 }
 # entry points that return a value instead of a status code
 VALUE_RETURNING = ('pvsg_xattn_num_splits', 'pvsg_gemm_bf16x3_packed_elems', 'pvsg_gemm_f16x2_packed_elems',
                    'pvsg_minvis_chain_workspace_bytes', 'pvsg_reconsdot_workspace_bytes', 'pvsg_rle_counts_to_chars',
                    'pvsg_decoder_rows_post_workspace_bytes', 'pvsg_tube_index_table_words', 'pvsg_conv1x1_stats_chunks',
                    'pvsg_conv3x3_stats_chunks', 'pvsg_rel_tail_workspace_bytes', 'pvsg_conv_slices', 'pvsg_rle_segments',
-                   'pvsg_rows_f16x2_packed_floats', 'pvsg_paged_attention_splits')
+                   'pvsg_rows_f16x2_packed_floats', 'pvsg_paged_attention_workspace_bytes')
 
 _lib = None
 
@@ -192,7 +192,7 @@ def load():
         f.restype = _ll if name in ('pvsg_gemm_bf16x3_packed_elems', 'pvsg_gemm_f16x2_packed_elems', 'pvsg_minvis_chain_workspace_bytes',
                                    'pvsg_decoder_rows_post_workspace_bytes', 'pvsg_reconsdot_workspace_bytes',
                                    'pvsg_rle_counts_to_chars', 'pvsg_tube_index_table_words', 'pvsg_rel_tail_workspace_bytes',
-                                   'pvsg_rows_f16x2_packed_floats') else _i
+                                   'pvsg_rows_f16x2_packed_floats', 'pvsg_paged_attention_workspace_bytes') else _i
         f.argtypes = argtypes
     _lib = lib
     try:                                    # loud, once: a second tenant on the GPU without a CU partition (parallel.py)

@@ -84,12 +84,15 @@ __device__ __forceinline__ void kv_store(unsigned char* p, const unsigned* w) {
 struct KvSpan {
   int len, there, fresh;
 };
-__device__ __forceinline__ KvSpan kv_span(const int* __restrict__ lens, const int* __restrict__ new_lens, int b, int T, int capacity) {
+__device__ __forceinline__ KvSpan kv_span_of(int len, int fresh, int T, int capacity) {
   KvSpan s;
-  s.len = max(lens[b], 0);
+  s.len = max(len, 0);
   s.there = min(s.len, capacity);
-  s.fresh = min(max(min(new_lens ? new_lens[b] : T, T), 0), s.len);
+  s.fresh = min(max(min(fresh, T), 0), s.len);
   return s;
+}
+__device__ __forceinline__ KvSpan kv_span(const int* __restrict__ lens, const int* __restrict__ new_lens, int b, int T, int capacity) {
+  return kv_span_of(lens[b], new_lens ? new_lens[b] : T, T, capacity);
 }
 
 __device__ __forceinline__ void kv_fault(int* faults, int bit) {

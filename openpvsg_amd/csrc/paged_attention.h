@@ -7,8 +7,12 @@
 // a row is dense in memory), and S^T leaves the pipe with a lane holding 4 keys of one query row -- which is the B operand of
 // O^T = V^T P^T as it stands, so P never moves.  For V^T a lane loads the same columns of several keys and pairs them by
 // byte permutes (16-bit products take 8 keys a lane; f32 products take one, and need no permutes).  Four waves take every
-// fourth tile and meet in LDS at the end; where few rows leave the card idle, `splits` workgroups share a cache and a second
-// kernel joins their (m, l, O).
+// fourth tile and meet in LDS at the end.
+//
+// Sequences differ in length, and only the device knows by how much.  So the tiles of all of them are one list, and as many
+// workgroups as the card holds each take an equal stretch of it: each finds its stretch by a scan over the lengths.  A (sequence, key
+// head, row group) that lies in several stretches leaves (m, l, O) of each, and a second kernel joins them.  Where no cache is
+// longer than a few tiles there is nothing to even out, and each has a workgroup of its own and no join.
 //
 // Rounding: 16-bit rows multiply in their own type, exact products in f32 sums; 8-bit codes convert to it exactly and their
 // scales multiply S and P in f32.  P goes to the matrix cores as a 16-bit high part plus a 16-bit rest (one part alone adds an error as
@@ -17,6 +21,8 @@
 // f32 or f16 pool run on the f32 products.
 #pragma once
 #include "kv_pages.h"
+
+#include <limits.h>
 
 #include <type_traits>
 
@@ -34,12 +40,28 @@ struct PagedAttn {
   long long table_stride, padding_stride;
   float scale_log2e;
   int width, padding_width, page_shift;
-  int B, T, q_heads, group, rows, row_groups, splits, chunk, causal;
+  int B, T, q_heads, group, rows, row_groups, causal;
+  int workgroups;                        // how many share the tiles; 0: one for each (sequence, key head, row group)
+  int* part_of;                          // of each: the sequence, the key head and row group, and the last workgroup that it splits with
 };
 
 constexpr int PA_WAVES = 4;
-constexpr int PA_MAX_CHUNK = 4096;
+constexpr int PA_CHUNK = 4096;           // keys whose pages are looked up at a time
+constexpr int PA_PART = 3;                // what a part costs beside its tiles, in tiles
+constexpr int PA_GRAIN = 2;               // tiles that a workgroup takes at least
 constexpr int PA_MAX_T = 32;
+
+// The kernel reads its arguments where the launch left them, again for each part of its work: held in scalar registers
+// throughout, they would push the loop's own values out of those (measured: 130 to 260 of them spilled).
+typedef const __attribute__((address_space(4))) PagedAttn PagedAttnArgs;
+
+// device memory that nothing writes while the kernel runs, read at a place that all threads share: by scalar loads
+__device__ __forceinline__ const __attribute__((address_space(4))) int* pa_const(const int* p) {
+  return (const __attribute__((address_space(4))) int*)p;
+}
+
+// workgroups of a CU that the kernel's registers leave room for
+constexpr int pa_per_cu(int dim, int tiles) { return dim <= 32 ? 4 : dim <= 64 ? (tiles == 1 ? 3 : 2) : dim <= 128 ? 2 : 1; }
 
 // four packed 16-bit words (the 8 elements of one lane of a matrix product's operand)
 template <int MT>
@@ -103,10 +125,10 @@ __device__ __forceinline__ void pa_store_row4(unsigned char* out, long long at, 
   }
 }
 
-// Rows r0 .. r1-1 of one (sequence, key head, split) by plain sums, a key at a time: the fallback for values that are not finite.
-// buf: 3 * 256 floats of LDS.
+// Rows r0 .. r1-1 of one (sequence, key head) over the keys lo .. hi-1, by plain sums, a key at a time: the fallback for values that are
+// not finite.  buf: 3 * 256 floats of LDS; part_o / part_ml: where a part goes, null for the result itself.
 template <int RT, int CT>
-__device__ void pa_rows_alone(const PagedAttn& a, int b, int h, int split, int r0, int r1, const KvSpan& span, float* buf) {
+__device__ void pa_rows_alone(PagedAttnArgs& a, int b, int h, int lo, int hi, int r0, int r1, const KvSpan& span, float* part_o, float* part_ml, float* buf) {
   const int tid = threadIdx.x, D = a.p.dim;
   int* page_of = reinterpret_cast<int*>(buf);                       // -1: not seen
   float *z_of = buf + 256, *w_of = buf + 512;
@@ -114,71 +136,67 @@ __device__ void pa_rows_alone(const PagedAttn& a, int b, int h, int split, int r
 #pragma unroll 1
   for (int r = r0; r < r1; ++r) {
     const int t = r / a.group, hq = h * a.group + r % a.group;
-    const int lim = t >= span.fresh ? 0 : a.causal ? min(span.len - span.fresh + t + 1, span.there) : span.there;
+    const int lim = t >= span.fresh ? 0 : min(hi, a.causal ? min(span.len - span.fresh + t + 1, span.there) : span.there);
     const unsigned char* qr = a.q + b * a.q_seq + t * a.q_token + (long long)hq * a.q_head;
     float top = -INFINITY, sum = 0.f, o = 0.f;
 #pragma unroll 1
-    for (long long c0 = (long long)split * a.chunk; c0 < lim; c0 += (long long)a.splits * a.chunk) {
-      const int c1 = (int)min(c0 + a.chunk, (long long)lim);
-#pragma unroll 1
-      for (int p0 = (int)c0; p0 < c1; p0 += 256) {
-        const int p = p0 + tid;
-        int page = -1;
-        if (p < c1 && (!a.padding || (p < a.padding_width && !a.padding[(long long)b * a.padding_stride + p]))) {
-          page = a.table[(long long)b * a.table_stride + (p >> a.page_shift)];
-          if ((unsigned)page >= (unsigned)a.p.num_pages) page = -1;
-        }
-        const int slot = p & (a.p.page_size - 1);
-        float z = -INFINITY;
-        if (page >= 0) {
-          const long long at = (long long)page * a.p.page_stride + (long long)h * a.p.head_stride + (long long)slot * a.p.slot_stride;
-          z = 0.f;
-          for (int d = 0; d < D; d += 8) {
-            unsigned kw[8], qw[8];
-            kv_load<kv_bytes(CT) == 4 ? 16 : kv_bytes(CT) * 8>(kw, static_cast<const unsigned char*>(a.p.k) + (at + d) * kv_bytes(CT));
-            if constexpr (kv_bytes(CT) == 4) kv_load<16>(kw + 4, static_cast<const unsigned char*>(a.p.k) + (at + d) * 4 + 16);
-            kv_load<16>(qw, qr + d * kv_bytes(RT));
-            if constexpr (kv_bytes(RT) == 4) kv_load<16>(qw + 4, qr + d * 4 + 16);
+    for (int p0 = lo; p0 < lim; p0 += 256) {
+      const int p = p0 + tid;
+      int page = -1;
+      if (p < lim && (!a.padding || (p < a.padding_width && !a.padding[(long long)b * a.padding_stride + p]))) {
+        page = a.table[(long long)b * a.table_stride + (p >> a.page_shift)];
+        if ((unsigned)page >= (unsigned)a.p.num_pages) page = -1;
+      }
+      const int slot = p & (a.p.page_size - 1);
+      float z = -INFINITY;
+      if (page >= 0) {
+        const long long at = (long long)page * a.p.page_stride + (long long)h * a.p.head_stride + (long long)slot * a.p.slot_stride;
+        z = 0.f;
+        for (int d = 0; d < D; d += 8) {
+          unsigned kw[8], qw[8];
+          kv_load<kv_bytes(CT) == 4 ? 16 : kv_bytes(CT) * 8>(kw, static_cast<const unsigned char*>(a.p.k) + (at + d) * kv_bytes(CT));
+          if constexpr (kv_bytes(CT) == 4) kv_load<16>(kw + 4, static_cast<const unsigned char*>(a.p.k) + (at + d) * 4 + 16);
+          kv_load<16>(qw, qr + d * kv_bytes(RT));
+          if constexpr (kv_bytes(RT) == 4) kv_load<16>(qw + 4, qr + d * 4 + 16);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) z += kv_elem<RT>(qw, i) * kv_elem<CT>(kw, i);
-          }
-          z *= a.scale_log2e;
-          if constexpr (kv_scaled(CT)) z *= a.p.k_scale[(long long)page * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + slot];
+          for (int i = 0; i < 8; ++i) z += kv_elem<RT>(qw, i) * kv_elem<CT>(kw, i);
         }
-        __syncthreads();                                            // the last block's lists have been read
-        page_of[tid] = page;
-        z_of[tid] = z;
-        __syncthreads();
-        float up = top;
-        for (int i = 0; i < 256; ++i) up = fmaxf(up, z_of[i]);
-        const float ref = up == -INFINITY ? 0.f : up;
-        const float shrink = __builtin_amdgcn_exp2f(top - ref);
-        top = up;
-        w_of[tid] = page < 0 ? 0.f : __builtin_amdgcn_exp2f(z - ref);
-        __syncthreads();
-        // (before anything was seen o and sum are 0, and shrink is 0 or 1)
-        o *= shrink, sum *= shrink;
-        for (int i = 0; i < min(256, c1 - p0); ++i) {
-          if (page_of[i] < 0) continue;
-          const int si = (p0 + i) & (a.p.page_size - 1);
-          const long long at = (long long)page_of[i] * a.p.page_stride + (long long)h * a.p.head_stride + (long long)si * a.p.slot_stride + dq;
-          const unsigned char* src = static_cast<const unsigned char*>(a.p.v) + at * kv_bytes(CT);
-          unsigned w[1];
-          if constexpr (kv_bytes(CT) == 4) w[0] = *reinterpret_cast<const unsigned*>(src);
-          else if constexpr (kv_bytes(CT) == 2) w[0] = *reinterpret_cast<const unsigned short*>(src);
-          else w[0] = *src;
-          float pv = w_of[i];
-          sum += pv;
-          if constexpr (kv_scaled(CT)) pv *= a.p.v_scale[(long long)page_of[i] * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + si];
-          o += pv * kv_elem<CT>(w, 0);
-        }
+        z *= a.scale_log2e;
+        if constexpr (kv_scaled(CT)) z *= a.p.k_scale[(long long)page * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + slot];
+      }
+      __syncthreads();                                            // the last block's lists have been read
+      page_of[tid] = page;
+      z_of[tid] = z;
+      __syncthreads();
+      float up = top;
+      for (int i = 0; i < 256; ++i) up = fmaxf(up, z_of[i]);
+      const float ref = up == -INFINITY ? 0.f : up;
+      const float shrink = __builtin_amdgcn_exp2f(top - ref);
+      top = up;
+      w_of[tid] = page < 0 ? 0.f : __builtin_amdgcn_exp2f(z - ref);
+      __syncthreads();
+      // (before anything was seen o and sum are 0, and shrink is 0 or 1)
+      o *= shrink, sum *= shrink;
+      for (int i = 0; i < min(256, lim - p0); ++i) {
+        if (page_of[i] < 0) continue;
+        const int si = (p0 + i) & (a.p.page_size - 1);
+        const long long at = (long long)page_of[i] * a.p.page_stride + (long long)h * a.p.head_stride + (long long)si * a.p.slot_stride + dq;
+        const unsigned char* src = static_cast<const unsigned char*>(a.p.v) + at * kv_bytes(CT);
+        unsigned w[1];
+        if constexpr (kv_bytes(CT) == 4) w[0] = *reinterpret_cast<const unsigned*>(src);
+        else if constexpr (kv_bytes(CT) == 2) w[0] = *reinterpret_cast<const unsigned short*>(src);
+        else w[0] = *src;
+        float pv = w_of[i];
+        sum += pv;
+        if constexpr (kv_scaled(CT)) pv *= a.p.v_scale[(long long)page_of[i] * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + si];
+        o += pv * kv_elem<CT>(w, 0);
       }
     }
     const long long row = ((long long)b * a.T + t) * a.q_heads + hq;
     if (tid < D) {
-      if (a.splits > 1) {
-        a.part_o[(row * a.splits + split) * D + tid] = o;
-        if (tid == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.splits + split) * 2) = make_float2(top, sum);
+      if (part_o) {
+        part_o[(r - r0) * D + tid] = o;
+        if (tid == 0) *reinterpret_cast<float2*>(part_ml + (r - r0) * 2) = make_float2(top, sum);
       } else {
         const float y = sum == 0.f ? 0.f : o / sum;
         if constexpr (RT == KV_F32) reinterpret_cast<float*>(a.out)[row * D + tid] = y;
@@ -199,7 +217,7 @@ __device__ __forceinline__ void pa_parts(float a, float b, unsigned (&w)[PARTS])
 }
 
 template <int RT, int CT, int DP, int NT, bool PADDED>
-__global__ __launch_bounds__(64 * PA_WAVES, DP <= 128 ? 2 : 1) void paged_attention_kernel(const PagedAttn a) {
+__global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attention_kernel(const PagedAttn) {
   constexpr bool M16 = RT != KV_F32 || CT == KV_BF16 || kv_scaled(CT);
   constexpr int QK = RT == KV_F16 ? KV_F16 : KV_BF16, PV = CT == KV_F16 ? KV_F16 : KV_BF16;      // operand types of the 16-bit products
   constexpr int QL = RT == KV_F32 ? 3 : 1, PL = RT == KV_F32 ? 3 : 2;
@@ -212,376 +230,429 @@ __global__ __launch_bounds__(64 * PA_WAVES, DP <= 128 ? 2 : 1) void paged_attent
   constexpr int QN = M16 ? DP / 32 : DP / 4;                        // steps of 8 packed columns, or single columns
   static_assert(!M16 || KC % 8 == 0, "16-bit products take 8 columns a lane");
 
-  __shared__ int s_page[PA_MAX_CHUNK / 8 + 1];
-  __shared__ __align__(16) unsigned char s_hide[PADDED ? PA_MAX_CHUNK : 16];
+  __shared__ int s_page[PA_CHUNK / 8 + 1];
+  __shared__ __align__(16) unsigned char s_hide[PADDED ? PA_CHUNK : 16];
   constexpr int OR = DP == 256 ? 8 : 16;                            // rows of a wave in LDS at a time
   __shared__ __align__(16) float s_o[PA_WAVES][OR][DP + 4];
   __shared__ float s_ml[PA_WAVES][16][2];
 
-  // which part of the work: the row groups of one (sequence, key head, split) run on one XCD and share its L2
-  unsigned unit = blockIdx.x, rg = 0;
-  if (a.row_groups > 1) {
-    const unsigned xcd = blockIdx.x & 7u, at = blockIdx.x >> 3;
-    unit = (at / a.row_groups) * 8u + xcd, rg = at % a.row_groups;
-  }
-  const unsigned heads = a.p.heads, bh = a.B * heads;
-  const int split = unit / bh;
-  if (split >= a.splits) return;
-  const int b = (unit % bh) / heads, h = unit % heads;
-  const int row0 = rg * (16 * NT);
-  const KvSpan span = kv_span(a.lens, a.new_lens, b, a.T, a.width << a.page_shift);
-  const int past = span.len - span.fresh;
-  // what the first and the last real row of this group see
-  const int t_lo = row0 / a.group, t_hi = min((min(row0 + 16 * NT, a.rows) - 1) / a.group, span.fresh - 1);
-  const int most = t_lo < span.fresh ? (a.causal ? min(past + t_hi + 1, span.there) : span.there) : 0;
-  const int least = a.causal ? min(past + t_lo + 1, span.there) : span.there;
-  const bool joined = a.splits > 1;
-  if (joined && (long long)split * a.chunk >= span.there) return;    // the join takes as many partials as there are chunks
+  constexpr int TILE = PA_WAVES * KEYS;
+  PagedAttnArgs* args = (PagedAttnArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+  auto tiles_of = [](int len, int capacity) { return max((min(max(len, 0), capacity) + TILE - 1) / TILE, 1); };   // one at least, which writes the zeros
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, m = lane & 15, g = lane >> 4;
-  const int D = a.p.dim, page_mask = a.p.page_size - 1;
-
-  // query rows, in the operand layout
-  unsigned qf[NT][QN * (M16 ? 4 * QL : 1)];
-  int lim[NT];
+  // ---- this workgroup's stretch.  The list: for each sequence its (key head, row group)s one after the other, each of them PA_PART
+  // entries that stand for what a part costs beside its tiles, then its tiles.  hr: the first one of sequence b that the stretch
+  // meets, `at` the entry of it where the stretch begins, `left` how many entries it has.
+  int b, hr, at, left, len;
+  unsigned share = 0, more = 0;                                     // workgroup i takes `share` entries, and one more if i < more
+  const int each = args->p.heads * args->row_groups;
+  if (PagedAttnArgs& a = *args; a.workgroups == 0) {
+    b = blockIdx.x / each, hr = blockIdx.x % each, at = 0;
+    len = pa_const(a.lens)[b];
+    left = INT_MAX;
+  } else {
+    // every wave scans the lengths by itself: 64 lanes, `per` sequences each
+    const int lane = threadIdx.x & 63, per = (a.B + 63) / 64, b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B), capacity = a.width << a.page_shift;
+    unsigned mine = 0;
+    for (int i = b0; i < b1; ++i) mine += PA_PART + tiles_of(a.lens[i], capacity);
+    mine *= each;
+    unsigned upto = mine;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = row0 + nt * 16 + m, t = r / a.group, j = r % a.group;
-    const bool real = r < a.rows && t < span.fresh;
-    lim[nt] = !real ? most : a.causal ? min(past + t + 1, span.there) : span.there;
-    const unsigned char* qr = a.q + b * a.q_seq + t * a.q_token + (long long)(h * a.group + j) * a.q_head;
-    constexpr int STEP = M16 ? 8 : 4;
-#pragma unroll
-    for (int i = 0; i < DP / 4 / STEP; ++i) {
-      const int d = (i * STEP / KC) * 4 * KC + KC * g + i * STEP % KC;
-      unsigned w[STEP * RB / 4] = {};
-      if (real && d < D) {
-        kv_load<16>(w, qr + d * RB);
-        if constexpr (STEP * RB == 32) kv_load<16>(w + 4, qr + d * RB + 16);
+    for (int o = 1; o < 64; o <<= 1) {
+      const unsigned x = __shfl_up(upto, o);
+      if (lane >= o) upto += x;
+    }
+    const unsigned total = __builtin_amdgcn_readlane(upto, 63);
+    const unsigned used = min((unsigned)a.workgroups, (total + PA_PART + PA_GRAIN - 1) / (PA_PART + PA_GRAIN));
+    share = total / used, more = total - share * used;
+    const unsigned first = blockIdx.x * share + min(blockIdx.x, more);
+    if (threadIdx.x == 0) a.part_of[3 * blockIdx.x] = -1;
+    if (blockIdx.x >= used) return;
+    left = share + (blockIdx.x < more ? 1 : 0);
+    const int whose = __builtin_ctzll(__ballot(first < upto));      // the lane whose sequences the stretch begins in
+    unsigned before = upto - mine;
+    b = b0;
+    if (per > 1) {
+      for (; b < b1 - 1; ++b) {
+        const unsigned n = (PA_PART + tiles_of(a.lens[b], capacity)) * each;
+        if (first < before + n) break;
+        before += n;
       }
+    }
+    b = __builtin_amdgcn_readlane(b, whose);
+    const unsigned inside = first - __builtin_amdgcn_readlane(before, whose);
+    len = pa_const(a.lens)[b];
+    const unsigned n = PA_PART + tiles_of(len, capacity);
+    hr = inside / n, at = inside - hr * n;
+  }
+
+#pragma unroll 1
+  for (bool next_b = false; left > 0; at = 0, next_b = ++hr == each, b += next_b, hr = next_b ? 0 : hr) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+s"(args), "+v"(tid));                        // (nothing made of these is kept from part to part)
+    PagedAttnArgs& a = *args;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), m = lane & 15, g = lane >> 4;
+    const int D = a.p.dim, page_mask = a.p.page_size - 1, capacity = a.width << a.page_shift;
+    if (next_b) len = pa_const(a.lens)[b];
+    const int tiles = tiles_of(len, capacity);
+    int tile0 = 0, tile1 = tiles;
+    if (a.workgroups) {
+      const int end = min(PA_PART + tiles, at + left);
+      tile0 = max(at - PA_PART, 0), tile1 = max(end - PA_PART, 0);
+      left -= end - at;
+      if (tile0 == tile1) continue;
+    } else {
+      left = 0;
+    }
+    const bool whole_row = tile0 == 0 && tile1 == tiles;
+    float *part_o = nullptr, *part_ml = nullptr;
+    if (!whole_row) {
+      // a stretch has one part at most that begins inside a row's tiles and one that only ends inside
+      const int slot = 2 * blockIdx.x + (tile0 == 0 ? 1 : 0);
+      part_o = a.part_o + (long long)slot * (16 * NT) * D;
+      part_ml = a.part_ml + (long long)slot * (16 * NT) * 2;
+      if (tile0 == 0 && tid == 0) {
+        // the workgroup that has the last tile: this stretch ends inside, so that one lies tiles - tile1 entries behind it
+        const unsigned end = (blockIdx.x + 1) * share + min(blockIdx.x + 1, more) + (tiles - tile1) - 1;
+        a.part_of[3 * blockIdx.x] = b, a.part_of[3 * blockIdx.x + 1] = hr;
+        a.part_of[3 * blockIdx.x + 2] = end < more * (share + 1) ? end / (share + 1) : more + (end - more * (share + 1)) / share;
+      }
+    }
+    const int h = hr / a.row_groups, row0 = hr % a.row_groups * (16 * NT);
+    const KvSpan span = kv_span_of(len, a.new_lens ? pa_const(a.new_lens)[b] : a.T, a.T, capacity);
+    const int past = span.len - span.fresh;
+    // what the first and the last real row of this group see
+    const int t_lo = row0 / a.group, t_hi = min((min(row0 + 16 * NT, a.rows) - 1) / a.group, span.fresh - 1);
+    const int most = min(t_lo < span.fresh ? (a.causal ? min(past + t_hi + 1, span.there) : span.there) : 0, (int)min((long long)tile1 * TILE, 1ll << 30));
+    const int least = a.causal ? min(past + t_lo + 1, span.there) : span.there;
+
+    // query rows, in the operand layout
+    unsigned qf[NT][QN * (M16 ? 4 * QL : 1)];
+    int lim[NT];
 #pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        if constexpr (M16 && QL > 1) {
-          unsigned part[QL];
-          pa_parts<QL, QK>(kv_elem<RT>(w, 2 * x), kv_elem<RT>(w, 2 * x + 1), part);
+    for (int nt = 0; nt < NT; ++nt) {
+      const int r = row0 + nt * 16 + m, t = r / a.group, j = r % a.group;
+      const bool real = r < a.rows && t < span.fresh;
+      lim[nt] = !real ? most : a.causal ? min(past + t + 1, span.there) : span.there;
+      const unsigned char* qr = a.q + b * a.q_seq + t * a.q_token + (long long)(h * a.group + j) * a.q_head;
+      constexpr int STEP = M16 ? 8 : 4;
 #pragma unroll
-          for (int l = 0; l < QL; ++l) qf[nt][(i * QL + l) * 4 + x] = part[l];
-        } else {
-          qf[nt][i * 4 + x] = w[x];
+      for (int i = 0; i < DP / 4 / STEP; ++i) {
+        const int d = (i * STEP / KC) * 4 * KC + KC * g + i * STEP % KC;
+        unsigned w[STEP * RB / 4] = {};
+        if (real && d < D) {
+          kv_load<16>(w, qr + d * RB);
+          if constexpr (STEP * RB == 32) kv_load<16>(w + 4, qr + d * RB + 16);
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          if constexpr (M16 && QL > 1) {
+            unsigned part[QL];
+            pa_parts<QL, QK>(kv_elem<RT>(w, 2 * x), kv_elem<RT>(w, 2 * x + 1), part);
+#pragma unroll
+            for (int l = 0; l < QL; ++l) qf[nt][(i * QL + l) * 4 + x] = part[l];
+          } else {
+            qf[nt][i * 4 + x] = w[x];
+          }
         }
       }
     }
-  }
 
-  f32x4 acc[NT][VE];
-  float mrow[NT], lrow[NT];
+    f32x4 acc[NT][VE];
+    float mrow[NT], lrow[NT];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    mrow[nt] = -INFINITY, lrow[nt] = 0.f;
+    for (int nt = 0; nt < NT; ++nt) {
+      mrow[nt] = -INFINITY, lrow[nt] = 0.f;
 #pragma unroll
-    for (int e = 0; e < VE; ++e) acc[nt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  const unsigned char* kbase = static_cast<const unsigned char*>(a.p.k) + (long long)h * a.p.head_stride * CB;
-  const unsigned char* vbase = static_cast<const unsigned char*>(a.p.v) + (long long)h * a.p.head_stride * CB;
-
-  // A tile's keys are loaded while the tile before is still in its softmax and its second product, its values while its own
-  // first product runs: each goes to the registers that the tile before has just done with, so nothing is held twice.
-  unsigned kw[KT][NK * KW], vw[KT * 4][NV * VW];
-  unsigned seen = 0;                                                // bit s*4+j: this lane's key 16 s + 4 g + j is there
-  float ks[KT][4], vs[KT][4];
-
-  for (long long c0 = (long long)split * a.chunk; c0 < most; c0 += (long long)a.splits * a.chunk) {
-    const int c1 = (int)min(c0 + a.chunk, (long long)most);
-    const int first_page = (int)(c0 >> a.page_shift);
-    __syncthreads();                                                // the previous chunk's pages have been read
-    for (int i = tid; i <= ((c1 - 1) >> a.page_shift) - first_page; i += 64 * PA_WAVES) {
-      int page = a.table[(long long)b * a.table_stride + first_page + i];
-      if ((unsigned)page >= (unsigned)a.p.num_pages) {
-        page = -1;
-        kv_fault(a.p.faults, 4);
-      }
-      s_page[i] = page;
+      for (int e = 0; e < VE; ++e) acc[nt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    if constexpr (PADDED) {
-      for (int i = tid; i < c1 - (int)c0; i += 64 * PA_WAVES) {
-        const int p = (int)c0 + i;
-        s_hide[i] = p < a.padding_width && !a.padding[(long long)b * a.padding_stride + p] ? 0 : 1;
-      }
-    }
-    __syncthreads();
+    const unsigned char* kbase = static_cast<const unsigned char*>(a.p.k) + (long long)h * a.p.head_stride * CB;
+    const unsigned char* vbase = static_cast<const unsigned char*>(a.p.v) + (long long)h * a.p.head_stride * CB;
 
-    // Keys past the end read their slot of the last page (in the pool, whatever it holds), keys of a bad page that of page 0;
-    // neither is seen.
-    auto load_k = [&](int k0) {
-#pragma unroll
-      for (int s = 0; s < KT; ++s) {
-        const int p = k0 + 16 * s + m;
-        const int page = max(s_page[(min(p, c1 - 1) >> a.page_shift) - first_page], 0);
-        const unsigned char* src = kbase + ((long long)page * a.p.page_stride + (long long)(p & page_mask) * a.p.slot_stride) * CB;
-#pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          const int d = i * 4 * KC + KC * g;
-          kv_load<KC * CB>(&kw[s][i * KW], src + (d < D ? d : 0) * CB);
+    // A tile's keys are loaded while the tile before is still in its softmax and its second product, its values while its own
+    // first product runs: each goes to the registers that the tile before has just done with, so nothing is held twice.
+    unsigned kw[KT][NK * KW], vw[KT * 4][NV * VW];
+    unsigned seen = 0;                                                // bit s*4+j: this lane's key 16 s + 4 g + j is there
+    float ks[KT][4], vs[KT][4];
+
+    for (int c0 = tile0 * TILE; c0 < most; c0 += PA_CHUNK) {
+      const int c1 = min(c0 + PA_CHUNK, most);
+      const int first_page = c0 >> a.page_shift;
+      __syncthreads();                                                // the previous chunk's pages have been read
+      for (int i = tid; i <= ((c1 - 1) >> a.page_shift) - first_page; i += 64 * PA_WAVES) {
+        int page = a.table[(long long)b * a.table_stride + first_page + i];
+        if ((unsigned)page >= (unsigned)a.p.num_pages) {
+          page = -1;
+          kv_fault(a.p.faults, 4);
+        }
+        s_page[i] = page;
+      }
+      if constexpr (PADDED) {
+        for (int i = tid; i < c1 - c0; i += 64 * PA_WAVES) {
+          const int p = c0 + i;
+          s_hide[i] = p < a.padding_width && !a.padding[(long long)b * a.padding_stride + p] ? 0 : 1;
         }
       }
-    };
-    auto load_v = [&](int k0) {
-      seen = 0;
+      __syncthreads();
+
+      // Keys past the end read their slot of the last page (in the pool, whatever it holds), keys of a bad page that of page 0;
+      // neither is seen.
+      auto load_k = [&](int k0) {
 #pragma unroll
-      for (int s = 0; s < KT; ++s) {
-        const int p = k0 + 16 * s + 4 * g;                          // four keys of one page
-        const int page = s_page[(min(p, c1 - 1) >> a.page_shift) - first_page], slot = p & page_mask;
-        unsigned there = page >= 0 ? (1u << min(max(c1 - p, 0), 4)) - 1u : 0u;
-        if constexpr (PADDED) {
-          const unsigned x = ~*reinterpret_cast<const unsigned*>(&s_hide[p < c1 ? p - (int)c0 : 0]);
-          there &= (x & 1u) | (x >> 7 & 2u) | (x >> 14 & 4u) | (x >> 21 & 8u);
-        }
-        seen |= there << (4 * s);
-        const unsigned char* src = vbase + ((long long)max(page, 0) * a.p.page_stride + (long long)slot * a.p.slot_stride) * CB;
+        for (int s = 0; s < KT; ++s) {
+          const int p = k0 + 16 * s + m;
+          const int page = max(s_page[(min(p, c1 - 1) >> a.page_shift) - first_page], 0);
+          const unsigned char* src = kbase + ((long long)page * a.p.page_stride + (long long)(p & page_mask) * a.p.slot_stride) * CB;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-          for (int c = 0; c < NV; ++c) {
-            const int d = c * 16 * VC + VC * m;
-            kv_load<VB>(&vw[4 * s + j][c * VW], src + (long long)j * a.p.slot_stride * CB + (d < D ? d : 0) * CB);
+          for (int i = 0; i < NK; ++i) {
+            const int d = i * 4 * KC + KC * g;
+            kv_load<KC * CB>(&kw[s][i * KW], src + (d < D ? d : 0) * CB);
           }
         }
-        if constexpr (kv_scaled(CT)) {
-          const long long at = (long long)max(page, 0) * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + slot;
-          kv_load<16>(reinterpret_cast<unsigned*>(ks[s]), reinterpret_cast<const unsigned char*>(a.p.k_scale + at));
-          kv_load<16>(reinterpret_cast<unsigned*>(vs[s]), reinterpret_cast<const unsigned char*>(a.p.v_scale + at));
-        }
-      }
-    };
-
-    // One tile, and the loads of the wave's next one where there is one: that is known to the compiler, since a wait for the
-    // values in flight must not depend on a branch over the loads behind them.  (Columns of K past the row's end hold other columns
-    // of it and meet zeros of Q; if those are not finite, neither is the result, see below.)
-    auto tile = [&](int k0, auto more) {
-      // ---- S^T = K Q^T
-      f32x4 st[NT][KT];
+      };
+      auto load_v = [&](int k0) {
+        seen = 0;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int s = 0; s < KT; ++s) st[nt][s] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < KT; ++s) {
-        if constexpr (M16) {
-#pragma unroll
-          for (int i = 0; i < QN; ++i) {
-            unsigned kf[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) kf[x] = CB == 2 ? kw[s][i * 4 + x] : pa_widen<QK, CT>(kw[s][(i * 4 + x) / 2], x & 1);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int l = 0; l < QL; ++l) {
-                const unsigned* qp = &qf[nt][(i * QL + l) * 4];
-                const unsigned qv[4] = {qp[0], qp[1], qp[2], qp[3]};
-                st[nt][s] = pa_mfma16<QK>(kf, qv, st[nt][s]);
-              }
+        for (int s = 0; s < KT; ++s) {
+          const int p = k0 + 16 * s + 4 * g;                          // four keys of one page
+          const int page = s_page[(min(p, c1 - 1) >> a.page_shift) - first_page], slot = p & page_mask;
+          unsigned there = page >= 0 ? (1u << min(max(c1 - p, 0), 4)) - 1u : 0u;
+          if constexpr (PADDED) {
+            const unsigned x = ~*reinterpret_cast<const unsigned*>(&s_hide[p < c1 ? p - c0 : 0]);
+            there &= (x & 1u) | (x >> 7 & 2u) | (x >> 14 & 4u) | (x >> 21 & 8u);
           }
-        } else {
+          seen |= there << (4 * s);
+          const unsigned char* src = vbase + ((long long)max(page, 0) * a.p.page_stride + (long long)slot * a.p.slot_stride) * CB;
 #pragma unroll
-          for (int i = 0; i < QN; ++i) {
-            const float kf = kv_elem<CT>(&kw[s][(i / KC) * KW], i % KC);
+          for (int j = 0; j < 4; ++j) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              st[nt][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf, __builtin_bit_cast(float, qf[nt][i]), st[nt][s], 0, 0, 0);
+            for (int c = 0; c < NV; ++c) {
+              const int d = c * 16 * VC + VC * m;
+              kv_load<VB>(&vw[4 * s + j][c * VW], src + (long long)j * a.p.slot_stride * CB + (d < D ? d : 0) * CB);
+            }
+          }
+          if constexpr (kv_scaled(CT)) {
+            const long long at = (long long)max(page, 0) * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + slot;
+            kv_load<16>(reinterpret_cast<unsigned*>(ks[s]), reinterpret_cast<const unsigned char*>(a.p.k_scale + at));
+            kv_load<16>(reinterpret_cast<unsigned*>(vs[s]), reinterpret_cast<const unsigned char*>(a.p.v_scale + at));
           }
         }
-      }
-      if constexpr (more.value) load_k(k0 + PA_WAVES * KEYS);
+      };
 
-      // ---- softmax: base 2, scale * log2(e) folded into S
-      const bool whole = !PADDED && k0 + KEYS <= least && __all(seen == (1u << (4 * KT)) - 1u);
-      float pr[NT][KT * 4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float z[KT * 4], top = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < KT * 4; ++k) {
-          z[k] = st[nt][k >> 2][k & 3] * a.scale_log2e;
-          if constexpr (kv_scaled(CT)) z[k] *= ks[k >> 2][k & 3];
-        }
-        if (!whole) {
-#pragma unroll
-          for (int k = 0; k < KT * 4; ++k) z[k] = ((seen >> k) & 1u) && k0 + 16 * (k >> 2) + 4 * g + (k & 3) < lim[nt] ? z[k] : -INFINITY;
-        }
-#pragma unroll
-        for (int k = 0; k < KT * 4; ++k) top = fmaxf(top, z[k]);
-        top = fmaxf(pa_max4(top), mrow[nt]);
-        const float ref = top == -INFINITY ? 0.f : top;             // a row that has seen nothing yet
-        if (__any(top > mrow[nt])) {
-          const float shrink = __builtin_amdgcn_exp2f(mrow[nt] - ref);
-          lrow[nt] *= shrink;
-#pragma unroll
-          for (int e = 0; e < VE; ++e) acc[nt][e] *= shrink;
-          mrow[nt] = top;
-        }
-#pragma unroll
-        for (int k = 0; k < KT * 4; ++k) {
-          pr[nt][k] = __builtin_amdgcn_exp2f(z[k] - ref);
-          lrow[nt] += pr[nt][k];
-        }
-        if constexpr (kv_scaled(CT)) {
-#pragma unroll
-          for (int k = 0; k < KT * 4; ++k) pr[nt][k] *= vs[k >> 2][k & 3];
-          if (!whole) {
-#pragma unroll
-            for (int k = 0; k < KT * 4; ++k) pr[nt][k] = z[k] != -INFINITY ? pr[nt][k] : 0.f;
-          }
-        }
-      }
-      if (!whole) {                                                 // a key that nobody sees must not meet the products
-#pragma unroll
-        for (int k = 0; k < KT * 4; ++k)
-#pragma unroll
-          for (int x = 0; x < NV * VW; ++x) vw[k][x] = (seen >> k) & 1u ? vw[k][x] : 0u;
-      }
-
-      // ---- O^T += V^T P^T
-      if constexpr (M16) {
-        unsigned pf[NT][PL][4];
+      // One tile, and the loads of the wave's next one where there is one: that is known to the compiler, since a wait for the
+      // values in flight must not depend on a branch over the loads behind them.  (Columns of K past the row's end hold other columns
+      // of it and meet zeros of Q; if those are not finite, neither is the result, see below.)
+      auto tile = [&](int k0, auto more) {
+        // ---- S^T = K Q^T
+        f32x4 st[NT][KT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            unsigned part[PL];
-            pa_parts<PL, PV>(pr[nt][2 * x], pr[nt][2 * x + 1], part);
+          for (int s = 0; s < KT; ++s) st[nt][s] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int l = 0; l < PL; ++l) pf[nt][l][x] = part[l];
+        for (int s = 0; s < KT; ++s) {
+          if constexpr (M16) {
+#pragma unroll
+            for (int i = 0; i < QN; ++i) {
+              unsigned kf[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) kf[x] = CB == 2 ? kw[s][i * 4 + x] : pa_widen<QK, CT>(kw[s][(i * 4 + x) / 2], x & 1);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int l = 0; l < QL; ++l) {
+                  const unsigned* qp = &qf[nt][(i * QL + l) * 4];
+                  const unsigned qv[4] = {qp[0], qp[1], qp[2], qp[3]};
+                  st[nt][s] = pa_mfma16<QK>(kf, qv, st[nt][s]);
+                }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < QN; ++i) {
+              const float kf = kv_elem<CT>(&kw[s][(i / KC) * KW], i % KC);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                st[nt][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf, __builtin_bit_cast(float, qf[nt][i]), st[nt][s], 0, 0, 0);
+            }
+          }
+        }
+        if constexpr (more.value) load_k(k0 + PA_WAVES * KEYS);
+
+        // ---- softmax: base 2, scale * log2(e) folded into S
+        const bool whole = !PADDED && k0 + KEYS <= least && __all(seen == (1u << (4 * KT)) - 1u);
+        float pr[NT][KT * 4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float z[KT * 4], top = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < KT * 4; ++k) {
+            z[k] = st[nt][k >> 2][k & 3] * a.scale_log2e;
+            if constexpr (kv_scaled(CT)) z[k] *= ks[k >> 2][k & 3];
+          }
+          if (!whole) {
+#pragma unroll
+            for (int k = 0; k < KT * 4; ++k) z[k] = ((seen >> k) & 1u) && k0 + 16 * (k >> 2) + 4 * g + (k & 3) < lim[nt] ? z[k] : -INFINITY;
           }
 #pragma unroll
-        for (int c = 0; c < NV; ++c) {
+          for (int k = 0; k < KT * 4; ++k) top = fmaxf(top, z[k]);
+          top = fmaxf(pa_max4(top), mrow[nt]);
+          const float ref = top == -INFINITY ? 0.f : top;             // a row that has seen nothing yet
+          if (__any(top > mrow[nt])) {
+            const float shrink = __builtin_amdgcn_exp2f(mrow[nt] - ref);
+            lrow[nt] *= shrink;
 #pragma unroll
-          for (int q4 = 0; q4 < (VC + 3) / 4; ++q4) {
-            // four columns (a pair of words of 16-bit elements, a word of codes) of eight keys -> one operand per column
-            unsigned vf[4][4];
+            for (int e = 0; e < VE; ++e) acc[nt][e] *= shrink;
+            mrow[nt] = top;
+          }
+#pragma unroll
+          for (int k = 0; k < KT * 4; ++k) {
+            pr[nt][k] = __builtin_amdgcn_exp2f(z[k] - ref);
+            lrow[nt] += pr[nt][k];
+          }
+          if constexpr (kv_scaled(CT)) {
+#pragma unroll
+            for (int k = 0; k < KT * 4; ++k) pr[nt][k] *= vs[k >> 2][k & 3];
+            if (!whole) {
+#pragma unroll
+              for (int k = 0; k < KT * 4; ++k) pr[nt][k] = z[k] != -INFINITY ? pr[nt][k] : 0.f;
+            }
+          }
+        }
+        if (!whole) {                                                 // a key that nobody sees must not meet the products
+#pragma unroll
+          for (int k = 0; k < KT * 4; ++k)
+#pragma unroll
+            for (int x = 0; x < NV * VW; ++x) vw[k][x] = (seen >> k) & 1u ? vw[k][x] : 0u;
+        }
+
+        // ---- O^T += V^T P^T
+        if constexpr (M16) {
+          unsigned pf[NT][PL][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              if constexpr (CB == 2) {
+              unsigned part[PL];
+              pa_parts<PL, PV>(pr[nt][2 * x], pr[nt][2 * x + 1], part);
 #pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                  if (4 * q4 + 2 * y < VC) {
-                    const unsigned wa = vw[2 * x][c * VW + 2 * q4 + y], wb = vw[2 * x + 1][c * VW + 2 * q4 + y];
-                    vf[2 * y][x] = __builtin_amdgcn_perm(wb, wa, 0x05040100u);
-                    vf[2 * y + 1][x] = __builtin_amdgcn_perm(wb, wa, 0x07060302u);
+              for (int l = 0; l < PL; ++l) pf[nt][l][x] = part[l];
+            }
+#pragma unroll
+          for (int c = 0; c < NV; ++c) {
+#pragma unroll
+            for (int q4 = 0; q4 < (VC + 3) / 4; ++q4) {
+              // four columns (a pair of words of 16-bit elements, a word of codes) of eight keys -> one operand per column
+              unsigned vf[4][4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                if constexpr (CB == 2) {
+#pragma unroll
+                  for (int y = 0; y < 2; ++y) {
+                    if (4 * q4 + 2 * y < VC) {
+                      const unsigned wa = vw[2 * x][c * VW + 2 * q4 + y], wb = vw[2 * x + 1][c * VW + 2 * q4 + y];
+                      vf[2 * y][x] = __builtin_amdgcn_perm(wb, wa, 0x05040100u);
+                      vf[2 * y + 1][x] = __builtin_amdgcn_perm(wb, wa, 0x07060302u);
+                    }
+                  }
+                } else {
+                  const unsigned wa = vw[2 * x][c * VW + q4], wb = vw[2 * x + 1][c * VW + q4];
+                  const unsigned t0 = __builtin_amdgcn_perm(wb, wa, 0x05010400u), t1 = __builtin_amdgcn_perm(wb, wa, 0x07030602u);
+                  vf[0][x] = pa_widen<PV, CT>(t0, false);
+                  vf[1][x] = pa_widen<PV, CT>(t0, true);
+                  if (VC > 2) {
+                    vf[2][x] = pa_widen<PV, CT>(t1, false);
+                    vf[3][x] = pa_widen<PV, CT>(t1, true);
                   }
                 }
-              } else {
-                const unsigned wa = vw[2 * x][c * VW + q4], wb = vw[2 * x + 1][c * VW + q4];
-                const unsigned t0 = __builtin_amdgcn_perm(wb, wa, 0x05010400u), t1 = __builtin_amdgcn_perm(wb, wa, 0x07030602u);
-                vf[0][x] = pa_widen<PV, CT>(t0, false);
-                vf[1][x] = pa_widen<PV, CT>(t0, true);
-                if (VC > 2) {
-                  vf[2][x] = pa_widen<PV, CT>(t1, false);
-                  vf[3][x] = pa_widen<PV, CT>(t1, true);
+              }
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                if (4 * q4 + y < VC) {
+                  const int e = c * VC + 4 * q4 + y;
+#pragma unroll
+                  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int l = 0; l < PL; ++l) acc[nt][e] = pa_mfma16<PV>(vf[y], pf[nt][l], acc[nt][e]);
                 }
               }
             }
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              if (4 * q4 + y < VC) {
-                const int e = c * VC + 4 * q4 + y;
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                  for (int l = 0; l < PL; ++l) acc[nt][e] = pa_mfma16<PV>(vf[y], pf[nt][l], acc[nt][e]);
-              }
-            }
           }
-        }
-      } else {
-#pragma unroll
-        for (int k = 0; k < KT * 4; ++k)
-#pragma unroll
-          for (int e = 0; e < VE; ++e) {
-            const float vf = kv_elem<CT>(&vw[k][(e / VC) * VW], e % VC);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) acc[nt][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, pr[nt][k], acc[nt][e], 0, 0, 0);
-          }
-      }
-      if constexpr (more.value) load_v(k0 + PA_WAVES * KEYS);
-    };
-
-    int k0 = (int)c0 + wave * KEYS;
-    if (k0 < c1) {
-      load_k(k0);
-      __builtin_amdgcn_sched_barrier(0);                            // keys first: the values are waited for later
-      load_v(k0);
-#pragma unroll 1
-      for (; k0 + PA_WAVES * KEYS < c1; k0 += PA_WAVES * KEYS) tile(k0, std::true_type{});
-      tile(k0, std::false_type{});
-    }
-  }
-
-  // What a row does not see must not reach it, but 0 * infinity and 0 * NaN do in a matrix product over shared values, and an
-  // infinite value meets the rest of its P, which may be 0 or negative.  So where a result is not finite, the rows are
-  // computed again, each from what it sees alone.
-  bool off = false;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int r = row0 + nt * 16 + m;
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < VE; ++e)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int d = (e / VC) * 16 * VC + VC * (4 * g + j) + e % VC;
-        bad |= d < D && !(__builtin_fabsf(acc[nt][e][j]) < INFINITY);
-      }
-    off |= bad && r < a.rows && r / a.group < span.fresh;
-  }
-  if (__syncthreads_or(off)) {
-    pa_rows_alone<RT, CT>(a, b, h, split, row0, min(row0 + 16 * NT, a.rows), span, &s_o[0][0][0]);
-    return;
-  }
-
-  // ---- the four waves' parts of each row
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const float l = pa_sum4(lrow[nt]);
-#pragma unroll
-    for (int half = 0; half < 16 / OR; ++half) {
-      __syncthreads();
-      if (g == 0) s_ml[wave][m][0] = mrow[nt], s_ml[wave][m][1] = l;
-      if (m / OR == half) {
-#pragma unroll
-        for (int e = 0; e < VE; ++e)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s_o[wave][m % OR][(e / VC) * 16 * VC + VC * (4 * g + j) + e % VC] = acc[nt][e][j];
-      }
-      __syncthreads();
-      for (int i = tid; i < OR * (DP / 4); i += 64 * PA_WAVES) {
-        const int ml = i / (DP / 4) + half * OR, d = (i % (DP / 4)) * 4;
-        const int r = row0 + nt * 16 + ml, t = r / a.group;
-        if (r >= a.rows || d >= D) continue;
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < PA_WAVES; ++w) top = fmaxf(top, s_ml[w][ml][0]);
-        const float ref = top == -INFINITY ? 0.f : top;
-        float sum = 0.f, o[4] = {};
-#pragma unroll
-        for (int w = 0; w < PA_WAVES; ++w) {
-          const float x = __builtin_amdgcn_exp2f(s_ml[w][ml][0] - ref);
-          sum += x * s_ml[w][ml][1];
-          const float4 v = ld4(&s_o[w][ml - half * OR][d]);
-          // a wave whose keys this row does not see adds nothing (its O is zero: no 0 * infinity comes of it)
-          o[0] += x * v.x, o[1] += x * v.y, o[2] += x * v.z, o[3] += x * v.w;
-        }
-        const long long row = ((long long)b * a.T + t) * a.q_heads + h * a.group + r % a.group;
-        if (joined) {
-          st4(a.part_o + (row * a.splits + split) * D + d, make_float4(o[0], o[1], o[2], o[3]));
-          if (d == 0) *reinterpret_cast<float2*>(a.part_ml + (row * a.splits + split) * 2) = make_float2(top, sum);
         } else {
-          const bool some = t < span.fresh && !(sum == 0.f);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) o[x] = some ? o[x] / sum : 0.f;
-          pa_store_row4<RT>(a.out, row * D + d, o);
+          for (int k = 0; k < KT * 4; ++k)
+#pragma unroll
+            for (int e = 0; e < VE; ++e) {
+              const float vf = kv_elem<CT>(&vw[k][(e / VC) * VW], e % VC);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) acc[nt][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf, pr[nt][k], acc[nt][e], 0, 0, 0);
+            }
+        }
+        if constexpr (more.value) load_v(k0 + PA_WAVES * KEYS);
+      };
+
+      int k0 = c0 + wave * KEYS;
+      if (k0 < c1) {
+        load_k(k0);
+        __builtin_amdgcn_sched_barrier(0);                            // keys first: the values are waited for later
+        load_v(k0);
+#pragma unroll 1
+        for (; k0 + PA_WAVES * KEYS < c1; k0 += PA_WAVES * KEYS) tile(k0, std::true_type{});
+        tile(k0, std::false_type{});
+      }
+    }
+
+    // ---- the four waves' parts of each row
+    bool off = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float l = pa_sum4(lrow[nt]);
+#pragma unroll
+      for (int half = 0; half < 16 / OR; ++half) {
+        __syncthreads();
+        if (g == 0) s_ml[wave][m][0] = mrow[nt], s_ml[wave][m][1] = l;
+        if (m / OR == half) {
+#pragma unroll
+          for (int e = 0; e < VE; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s_o[wave][m % OR][(e / VC) * 16 * VC + VC * (4 * g + j) + e % VC] = acc[nt][e][j];
+        }
+        __syncthreads();
+        for (int i = tid; i < OR * (DP / 4); i += 64 * PA_WAVES) {
+          const int ml = i / (DP / 4) + half * OR, d = (i % (DP / 4)) * 4;
+          const int r = row0 + nt * 16 + ml, t = r / a.group;
+          if (r >= a.rows || d >= D) continue;
+          float top = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < PA_WAVES; ++w) top = fmaxf(top, s_ml[w][ml][0]);
+          const float ref = top == -INFINITY ? 0.f : top;
+          float sum = 0.f, o[4] = {};
+#pragma unroll
+          for (int w = 0; w < PA_WAVES; ++w) {
+            const float x = __builtin_amdgcn_exp2f(s_ml[w][ml][0] - ref);
+            sum += x * s_ml[w][ml][1];
+            const float4 v = ld4(&s_o[w][ml - half * OR][d]);
+            // a wave whose keys this row does not see adds nothing (its O is zero: no 0 * infinity comes of it)
+            o[0] += x * v.x, o[1] += x * v.y, o[2] += x * v.z, o[3] += x * v.w;
+          }
+          const long long row = ((long long)b * a.T + t) * a.q_heads + h * a.group + r % a.group;
+          off |= t < span.fresh && !(__builtin_fabsf(o[0]) + __builtin_fabsf(o[1]) + __builtin_fabsf(o[2]) + __builtin_fabsf(o[3]) < INFINITY);
+          if (part_o) {
+            st4(part_o + (nt * 16 + ml) * D + d, make_float4(o[0], o[1], o[2], o[3]));
+            if (d == 0) *reinterpret_cast<float2*>(part_ml + (nt * 16 + ml) * 2) = make_float2(top, sum);
+          } else {
+            const bool some = t < span.fresh && !(sum == 0.f);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[x] = some ? o[x] / sum : 0.f;
+            pa_store_row4<RT>(a.out, row * D + d, o);
+          }
         }
       }
     }
+    // What a row does not see must not reach it, but 0 * infinity and 0 * NaN do in a matrix product over shared values, and an
+    // infinite value meets the rest of its P, which may be 0 or negative.  So where a result is not finite, the rows are
+    // computed again, each from what it sees alone.  (The barrier also parts these rows' LDS from the next ones'.)
+    if (__syncthreads_or(off))
+      pa_rows_alone<RT, CT>(a, b, h, tile0 * TILE, most, row0, min(row0 + 16 * NT, a.rows), span, part_o, part_ml, &s_o[0][0][0]);
   }
 }
 

@@ -3,69 +3,112 @@
 
 namespace pvsg {
 
-// The join: one workgroup per query row, dim / 4 threads across a partial and the others down the splits.
+// The join: workgroup i looks at the part that workgroup i of the first kernel left of a (sequence, key head, row group) that ends in a
+// later stretch, and adds the parts of the stretches up to that one.  dim / 4 threads across a row; of the groups of so many
+// threads, `share` take one row's parts between them, so that few rows of many parts are read at once as well.
 template <int RT>
-__global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAttn a) {
-  const long long row = blockIdx.x;
-  const int b = (int)(row / ((long long)a.T * a.q_heads)), t = (int)(row / a.q_heads % a.T);
+__global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAttn a, int tile_rows) {
+  const int first = blockIdx.x, b = a.part_of[3 * first];
+  if (b < 0) return;
+  const int hr = a.part_of[3 * first + 1], n = a.part_of[3 * first + 2] - first + 1;
   const KvSpan span = kv_span(a.lens, a.new_lens, b, a.T, a.width << a.page_shift);
-  const int n = t < span.fresh ? (int)min((long long)a.splits, ((long long)span.there + a.chunk - 1) / a.chunk) : 0;
-  const int D = a.p.dim, d4 = D / 4, down = 256 / d4;
-  const int x = threadIdx.x % d4, s0 = threadIdx.x / d4;
-  const float* ml = a.part_ml + row * a.splits * 2;
-  float top = -INFINITY;
-  for (int s = threadIdx.x & 63; s < n; s += 64) top = fmaxf(top, ml[2 * s]);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  const float ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (s0 < down) {
-    for (int s = s0; s < n; s += down) {
-      const float2 p = *reinterpret_cast<const float2*>(ml + 2 * s);
-      const float w = __builtin_amdgcn_exp2f(p.x - ref);
-      const float4 v = ld4(a.part_o + (row * a.splits + s) * D + 4 * x);
-      sum += w * p.y;
-      o.x += w * v.x, o.y += w * v.y, o.z += w * v.z, o.w += w * v.w;
-    }
-  }
+  const int h = hr / a.row_groups, row0 = hr % a.row_groups * tile_rows, rows = min(tile_rows, a.rows - row0);
+  const int D = a.p.dim, d4 = D / 4, groups = 256 / d4, x = threadIdx.x % d4, y = threadIdx.x / d4;
+  const int share = max(1, min(groups / rows, n / 2)), at_once = groups / share;
   __shared__ __align__(16) float s_o[256][4];
-  __shared__ float s_l[256];
-  st4(s_o[threadIdx.x], o);
-  s_l[threadIdx.x] = sum;
-  __syncthreads();
-  if (threadIdx.x < (unsigned)d4) {
-    for (int s = 1; s < down; ++s) {
-      const float4 v = ld4(s_o[s * d4 + x]);
-      o.x += v.x, o.y += v.y, o.z += v.z, o.w += v.w;
-      sum += s_l[s * d4 + x];
+  __shared__ float s_m[256], s_l[256];
+  for (int r0 = 0; r0 < rows; r0 += at_once) {
+    const int r = r0 + y / share, k0 = y % share;
+    const bool mine = y < at_once * share && r < rows;
+    // part k: what the first stretch left at its end, then what each later one left at its beginning
+    float top = -INFINITY, sum = 0.f, o[4] = {};
+    if (mine) {
+#pragma unroll 4
+      for (int k = k0; k < n; k += share) {
+        const long long slot = (long long)(2 * (first + k) + (k == 0 ? 1 : 0)) * tile_rows + r;
+        const float2 p = *reinterpret_cast<const float2*>(a.part_ml + 2 * slot);
+        const float4 v = ld4(a.part_o + slot * D + 4 * x);
+        const float up = fmaxf(top, p.x), ref = up == -INFINITY ? 0.f : up;
+        const float keep = __builtin_amdgcn_exp2f(top - ref), w = __builtin_amdgcn_exp2f(p.x - ref);
+        sum = sum * keep + w * p.y;
+        o[0] = o[0] * keep + w * v.x, o[1] = o[1] * keep + w * v.y, o[2] = o[2] * keep + w * v.z, o[3] = o[3] * keep + w * v.w;
+        top = up;
+      }
     }
-    const bool some = !(sum == 0.f);
-    const float y[4] = {some ? o.x / sum : 0.f, some ? o.y / sum : 0.f, some ? o.z / sum : 0.f, some ? o.w / sum : 0.f};
-    pa_store_row4<RT>(a.out, row * D + 4 * x, y);
+    if (share > 1) {
+      __syncthreads();
+      st4(s_o[threadIdx.x], make_float4(o[0], o[1], o[2], o[3]));
+      s_m[threadIdx.x] = top, s_l[threadIdx.x] = sum;
+      __syncthreads();
+      if (mine && k0 == 0) {
+        float up = top;
+        for (int s = 1; s < share; ++s) up = fmaxf(up, s_m[threadIdx.x + s * d4]);
+        const float ref = up == -INFINITY ? 0.f : up, keep = __builtin_amdgcn_exp2f(top - ref);
+        sum *= keep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] *= keep;
+        for (int s = 1; s < share; ++s) {
+          const float w = __builtin_amdgcn_exp2f(s_m[threadIdx.x + s * d4] - ref);
+          const float4 v = ld4(s_o[threadIdx.x + s * d4]);
+          sum += w * s_l[threadIdx.x + s * d4];
+          o[0] += w * v.x, o[1] += w * v.y, o[2] += w * v.z, o[3] += w * v.w;
+        }
+      }
+    }
+    if (mine && k0 == 0) {
+      const int t = (row0 + r) / a.group;
+      const bool some = t < span.fresh && !(sum == 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = some ? o[i] / sum : 0.f;
+      pa_store_row4<RT>(a.out, (((long long)b * a.T + t) * a.q_heads + h * a.group + (row0 + r) % a.group) * D + 4 * x, o);
+    }
   }
 }
+
+// caches of up to so many tiles are not split: each has a workgroup of its own
+constexpr int PA_SHORT = 4;
 
 // 16-row tiles a wave carries: two where there are more rows than one tile holds and the accumulators of two fit
 static int pa_tiles(int rows, int dim, int row_type) { return rows > 16 && dim <= (row_type == KV_F32 ? 64 : 128) ? 2 : 1; }
 
+// How the work is shared out: rows of a tile group, groups, and how many workgroups take equal stretches (0: one each)
+struct PaPlan {
+  int tiles, row_groups, workgroups;
+  long long units;
+  size_t part_o, part_ml, part_of;       // floats, floats, ints of the workspace
+};
+static PaPlan pa_plan(const pvsg_kv_pages& p, int B, int T, int q_heads, int row_type, int table_width, long long max_len) {
+  PaPlan s{};
+  const int rows = T * (q_heads / p.heads);
+  s.tiles = pa_tiles(rows, p.dim, row_type);
+  s.row_groups = (rows + 16 * s.tiles - 1) / (16 * s.tiles);
+  s.units = (long long)B * p.heads * s.row_groups;
+  const long long capacity = (long long)table_width * p.page_size, longest = max_len > 0 && max_len < capacity ? max_len : capacity;
+  const bool f32_products = row_type == KV_F32 && (p.type == KV_F32 || p.type == KV_F16);
+  const int tile = PA_WAVES * (f32_products && p.dim > 32 ? 16 : 32);
+  const long long tiles = (longest + tile - 1) / tile;
+  if (tiles <= PA_SHORT || s.units * (capacity / tile + 1 + PA_PART) >= (1ll << 31)) return s;     // (the list is counted in 32 bits)
+  const long long room = 256 * pa_per_cu(p.dim, s.tiles), work = (s.units * (tiles + PA_PART) + PA_PART + PA_GRAIN - 1) / (PA_PART + PA_GRAIN);
+  s.workgroups = (int)(work < room ? work : room);
+  const size_t rows_of = (size_t)2 * s.workgroups * 16 * s.tiles;
+  s.part_o = rows_of * p.dim, s.part_ml = rows_of * 2, s.part_of = (size_t)3 * s.workgroups;
+  return s;
+}
+
 }  // namespace pvsg
 
-extern "C" int pvsg_paged_attention_splits(int B, int T, int q_heads, int kv_heads, int dim, int row_type, long long max_len) {
+extern "C" long long pvsg_paged_attention_workspace_bytes(const pvsg_kv_pages* pages, int B, int T, int q_heads, int row_type, int table_width,
+                                                          long long max_len) {
   using namespace pvsg;
-  if (B <= 0 || T <= 0 || kv_heads <= 0 || q_heads < kv_heads || max_len <= 0) return 1;
-  const int rows = T * (q_heads / kv_heads), per = 16 * pa_tiles(rows, dim, row_type);
-  const long long units = (long long)B * kv_heads * ((rows + per - 1) / per);
-  const long long tiles = (max_len + 127) / 128;                    // one 32-key tile for each wave
-  long long n = (2048 + units - 1) / units;
-  n = n < tiles ? n : tiles;
-  return (int)(n < 1 ? 1 : n > 512 ? 512 : n);
+  if (!pages || pages->heads <= 0 || pages->dim <= 0 || B <= 0 || T <= 0 || q_heads < pages->heads || table_width <= 0) return 0;
+  const PaPlan s = pa_plan(*pages, B, T, q_heads, row_type, table_width, max_len);
+  return (long long)(s.part_o + s.part_ml + s.part_of) * 4;
 }
 
 extern "C" int pvsg_paged_attention(const pvsg_kv_pages* pages, const void* q, long long q_seq_stride, long long q_token_stride,
                                     long long q_head_stride, void* out, int row_type, const int* table, long long table_stride, int table_width,
                                     const int* lens, const int* new_lens, const uint8_t* padding, long long padding_stride, int padding_width,
-                                    int B, int T, int q_heads, float scale, int causal, long long max_len, int splits, void* workspace, void* stream) {
+                                    int B, int T, int q_heads, float scale, int causal, long long max_len, void* workspace, void* stream) {
   using namespace pvsg;
   if (const int rc = kv_check_pages("pvsg_paged_attention", pages, table, table_stride, table_width, lens, B)) return rc;
   PVSG_REQUIRE(q && out, "pvsg_paged_attention: null pointer");
@@ -75,9 +118,12 @@ extern "C" int pvsg_paged_attention(const pvsg_kv_pages* pages, const void* q, l
   PVSG_REQUIRE(((q_seq_stride | q_token_stride | q_head_stride) * rb) % 16 == 0 && (((uintptr_t)q | (uintptr_t)out) & 15) == 0, "pvsg_paged_attention: rows are not 16-byte aligned");
   PVSG_REQUIRE(T >= 0 && T <= PA_MAX_T, "pvsg_paged_attention: %d new tokens (at most %d)", T, PA_MAX_T);
   PVSG_REQUIRE(q_heads > 0 && q_heads % pages->heads == 0 && q_heads / pages->heads <= 1024, "pvsg_paged_attention: %d query heads over %d key heads", q_heads, pages->heads);
-  PVSG_REQUIRE(splits >= 1 && splits <= 512 && (splits == 1 || (workspace && ((uintptr_t)workspace & 15) == 0)), "pvsg_paged_attention: %d splits, workspace %p", splits, workspace);
   PVSG_REQUIRE(!padding || (padding_width >= 0 && padding_stride >= 0), "pvsg_paged_attention: bad padding mask");
   if (B == 0 || T == 0) return PVSG_OK;
+  const PaPlan s = pa_plan(*pages, B, T, q_heads, row_type, table_width, max_len);
+  PVSG_REQUIRE(s.workgroups == 0 || (workspace && ((uintptr_t)workspace & 15) == 0), "pvsg_paged_attention: workspace %p, %lld bytes are needed", workspace,
+               (long long)(s.part_o + s.part_ml + s.part_of) * 4);
+  PVSG_REQUIRE(s.units < (1ll << 31), "pvsg_paged_attention: %lld parts are too many for one launch", s.units);
   PagedAttn a{};
   a.p = *pages;
   a.q = static_cast<const unsigned char*>(q), a.out = static_cast<unsigned char*>(out);
@@ -87,27 +133,21 @@ extern "C" int pvsg_paged_attention(const pvsg_kv_pages* pages, const void* q, l
   a.scale_log2e = scale * 1.44269504088896340736f;
   a.width = table_width, a.padding_width = padding_width;
   while ((1 << a.page_shift) < pages->page_size) ++a.page_shift;
-  a.B = B, a.T = T, a.q_heads = q_heads, a.group = q_heads / pages->heads, a.rows = T * a.group, a.splits = splits, a.causal = causal;
-  const int tiles = pa_tiles(a.rows, pages->dim, row_type);
-  a.row_groups = (a.rows + 16 * tiles - 1) / (16 * tiles);
-  const long long capacity = (long long)table_width * pages->page_size;
-  const long long longest = max_len > 0 && max_len < capacity ? max_len : capacity;
-  const long long share = ((longest + splits - 1) / splits + 127) / 128 * 128;
-  a.chunk = (int)(share < PA_MAX_CHUNK ? share : PA_MAX_CHUNK);
-  const long long total = (long long)B * T * q_heads;
-  a.part_o = static_cast<float*>(workspace);
-  a.part_ml = a.part_o ? a.part_o + total * splits * pages->dim : nullptr;
-  long long units = (long long)B * pages->heads * splits;
-  if (a.row_groups > 1) units = (units + 7) / 8 * 8 * a.row_groups;
-  PVSG_REQUIRE(units < (1ll << 31) && total < (1ll << 31), "pvsg_paged_attention: too many rows for one launch");
+  a.B = B, a.T = T, a.q_heads = q_heads, a.group = q_heads / pages->heads, a.rows = T * a.group, a.row_groups = s.row_groups, a.causal = causal;
+  a.workgroups = s.workgroups;
+  if (s.workgroups) {
+    a.part_o = static_cast<float*>(workspace);
+    a.part_ml = a.part_o + s.part_o;
+    a.part_of = reinterpret_cast<int*>(a.part_ml + s.part_ml);
+  }
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  const unsigned blocks = (unsigned)units;
-  (row_type == KV_F32 ? pa_run_f32 : row_type == KV_BF16 ? pa_run_bf16 : pa_run_f16)(a, tiles, blocks, st);
+  (row_type == KV_F32 ? pa_run_f32 : row_type == KV_BF16 ? pa_run_bf16 : pa_run_f16)(a, s.tiles, (unsigned)(s.workgroups ? s.workgroups : s.units), st);
   PVSG_LAUNCH_CHECK("pvsg_paged_attention");
-  if (splits > 1) {
-    if (row_type == KV_F32) hipLaunchKernelGGL((paged_attention_join_kernel<KV_F32>), dim3((unsigned)total), dim3(256), 0, st, a);
-    else if (row_type == KV_BF16) hipLaunchKernelGGL((paged_attention_join_kernel<KV_BF16>), dim3((unsigned)total), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((paged_attention_join_kernel<KV_F16>), dim3((unsigned)total), dim3(256), 0, st, a);
+  if (s.workgroups > 1) {
+    const dim3 grid((unsigned)(s.workgroups - 1));
+    if (row_type == KV_F32) hipLaunchKernelGGL((paged_attention_join_kernel<KV_F32>), grid, dim3(256), 0, st, a, 16 * s.tiles);
+    else if (row_type == KV_BF16) hipLaunchKernelGGL((paged_attention_join_kernel<KV_BF16>), grid, dim3(256), 0, st, a, 16 * s.tiles);
+    else hipLaunchKernelGGL((paged_attention_join_kernel<KV_F16>), grid, dim3(256), 0, st, a, 16 * s.tiles);
     PVSG_LAUNCH_CHECK("pvsg_paged_attention");
   }
   return PVSG_OK;

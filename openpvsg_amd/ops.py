@@ -1792,15 +1792,13 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
         return out.zero_()
     if B == 0 or T == 0:
         return out
-    longest = table.shape[1] * pages.page_size
-    if max_len is not None:
-        longest = max(1, min(longest, int(max_len)))
-    splits = _lib.load().pvsg_paged_attention_splits(B, T, HQ, pages.heads, D, _KV_ROW_TYPES[q.dtype], longest)
-    work = torch.empty((B * T * HQ * splits * (D + 2),), device=q.device, dtype=torch.float32) if splits > 1 else None
+    width, row, longest = table.shape[1], _KV_ROW_TYPES[q.dtype], 0 if max_len is None else max(1, int(max_len))
+    nbytes = _lib.load().pvsg_paged_attention_workspace_bytes(pages._struct, B, T, HQ, row, width, longest)
+    work = torch.empty((nbytes,), device=q.device, dtype=torch.uint8) if nbytes else None
     sb, st, sh, _ = q.stride()
     with _on(pages.device):
-        _lib.call('pvsg_paged_attention', pages._struct, q.data_ptr(), sb, st, sh, out.data_ptr(), _KV_ROW_TYPES[q.dtype], table.data_ptr(),
-                  table.stride(0), table.shape[1], lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None,
-                  mask.data_ptr() if mask is not None else None, ms, mw, B, T, HQ, D ** -0.5 if scale is None else float(scale),
-                  1 if causal else 0, longest, splits, work.data_ptr() if work is not None else None, _stream_ptr())
+        _lib.call('pvsg_paged_attention', pages._struct, q.data_ptr(), sb, st, sh, out.data_ptr(), row, table.data_ptr(), table.stride(0), width,
+                  lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, mask.data_ptr() if mask is not None else None,
+                  ms, mw, B, T, HQ, D ** -0.5 if scale is None else float(scale), 1 if causal else 0, longest,
+                  work.data_ptr() if work is not None else None, _stream_ptr())
     return out

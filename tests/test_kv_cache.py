@@ -149,7 +149,7 @@ def test_bad_pools_are_refused(hip_lib, bad):
     p, one = pages_struct(**bad), ctypes.c_void_p(4096)
     assert hip_lib.pvsg_kv_append(p, one, one, 0, 64, 64, 64, one, 2, 2, one, None, 1, 1, None) == 1
     assert hip_lib.pvsg_kv_read(p, one, one, 0, one, 2, 2, one, 1, 0, 4, None) == 1
-    assert hip_lib.pvsg_paged_attention(p, one, 64, 64, 64, one, 0, one, 2, 2, one, None, None, 0, 0, 1, 1, 4, 1.0, 1, 0, 1, None, None) == 1
+    assert hip_lib.pvsg_paged_attention(p, one, 64, 64, 64, one, 0, one, 2, 2, one, None, None, 0, 0, 1, 1, 4, 1.0, 1, 0, None, None) == 1
     assert len(hip_lib.pvsg_last_error()) > 10
 
 
@@ -162,29 +162,31 @@ def test_bad_calls_are_refused(hip_lib):
     def read(out=one, kind=0, B=1, start=0, length=4):
         return hip_lib.pvsg_kv_read(p, out, one, kind, one, 2, 2, one, B, start, length, None)
 
-    def attend(pool=p, q=one, out=one, row=0, T=1, HQ=4, splits=1, work=None, st=(64, 64, 64), B=1):
-        return hip_lib.pvsg_paged_attention(pool, q, *st, out, row, one, 2, 2, one, None, None, 0, 0, B, T, HQ, 1.0, 1, 0, splits, work, None)
+    def attend(pool=p, q=one, out=one, row=0, T=1, HQ=4, width=2, work=None, st=(64, 64, 64), B=1):
+        return hip_lib.pvsg_paged_attention(pool, q, *st, out, row, one, width, width, one, None, None, 0, 0, B, T, HQ, 1.0, 1, 0, work, None)
 
     for rc in (append(k=None), append(row=3), append(st=(64, 64, 66)), append(table=None), append(width=0), append(width=1 << 27), append(lens=None),
                append(B=-1), append(B=70000), append(T=-1), append(k=ctypes.c_void_p(4100)),
                read(out=None), read(kind=4), read(B=-2), read(start=-1), read(length=-1), read(out=ctypes.c_void_p(4104)),
-               attend(q=None), attend(out=None), attend(row=5), attend(T=33), attend(HQ=6), attend(HQ=0), attend(splits=0), attend(splits=513),
-               attend(splits=2), attend(splits=2, work=ctypes.c_void_p(4100)), attend(st=(64, 66, 64)), attend(row=1),
+               attend(q=None), attend(out=None), attend(row=5), attend(T=33), attend(HQ=6), attend(HQ=0),
+               attend(width=5000), attend(width=5000, work=ctypes.c_void_p(4100)), attend(st=(64, 66, 64)), attend(row=1),
                attend(pool=pages_struct(type=2), row=1), attend(pool=pages_struct(type=1), row=2)):
         assert rc == 1, hip_lib.pvsg_last_error()
     # nothing to do is no error and launches nothing
     assert append(B=0) == 0 and append(T=0) == 0 and read(length=0) == 0 and read(B=0) == 0 and attend(B=0) == 0 and attend(T=0) == 0
 
 
-def test_splits_fill_the_card_and_stay_in_range(hip_lib):
-    f = hip_lib.pvsg_paged_attention_splits
-    assert f(1, 1, 4, 4, 128, 0, 1) == 1 and f(0, 1, 4, 4, 128, 0, 100) == 1
+def test_workspace_is_bounded_by_the_card(hip_lib):
+    """none where every cache is a few tiles, and two parts for each of at most 1024 workgroups however long the caches are"""
+    def f(B=1, T=1, HQ=4, row=0, width=1, longest=0, **kw):
+        return hip_lib.pvsg_paged_attention_workspace_bytes(pages_struct(**kw), B, T, HQ, row, width, longest)
+    assert f() == 0 and f(width=1000, longest=1) == 0 and f(B=0, width=1000) == 0
     last = 0
-    for n in (1, 128, 129, 1000, 65536, 1 << 30):
-        s = f(1, 1, 8, 8, 128, 1, n)
-        assert 1 <= s <= 512 and s >= last and s <= -(-n // 128)
-        last = s
-    assert f(256, 1, 64, 8, 128, 1, 65536) <= f(1, 1, 64, 8, 128, 1, 65536)
+    for width in (64, 1000, 4096, 1 << 20):
+        n = f(width=width)
+        assert last <= n <= 2 * 1024 * 32 * (64 + 2) * 4 + 3 * 1024 * 4
+        last = n
+    assert f(B=60000, T=32, HQ=64, width=1 << 20) <= 2 * 1024 * 32 * (64 + 2) * 4 + 3 * 1024 * 4
 
 
 def test_cpu_tensors_are_refused(hip_lib):
