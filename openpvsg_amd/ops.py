@@ -1662,41 +1662,50 @@ class KVPages:
         return cls(k, v, *(torch.empty((num_pages, heads, page_size), device=device) for _ in range(2)))
 
 
-def _kv_ints(t, name, pages, shape):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.device != pages.device or t.dim() != len(shape) or \
-            any(n is not None and n != m for n, m in zip(shape, t.shape)):
-        raise RuntimeError('%s must be an int32 tensor of shape %s on %s' % (name, tuple('?' if n is None else n for n in shape), pages.device))
-    return t if t.stride(-1) == 1 else t.contiguous()
+def _kv_ints(t, name, pages, B):
+    """(B,) int32 on the pool's device, dense"""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != pages.device or t.shape != (B,):
+        raise RuntimeError('%s must be an int32 tensor of shape (%d,) on %s' % (name, B, pages.device))
+    return t if B < 2 or t.stride(0) == 1 else t.contiguous()
 
 
-def _kv_table(table, pages, B):
-    t = _kv_ints(table, 'table', pages, (B, None))
-    if t.shape[1] < 1 or t.shape[1] * pages.page_size > 1 << 30:
-        raise RuntimeError('table: %d pages of %d positions (one page at least, 2^30 positions at most)' % (t.shape[1], pages.page_size))
-    return t
+def _kv_table(t, pages, B):
+    """(B, W) int32 page table with dense rows -> tensor, row stride, W"""
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != pages.device or t.dim() != 2 or B not in (None, t.shape[0]):
+        raise RuntimeError('table must be an int32 tensor of shape (%s, pages) on %s' % ('?' if B is None else B, pages.device))
+    W = t.shape[1]
+    if W < 1 or W * pages.page_size > 1 << 30:
+        raise RuntimeError('table: %d pages of %d positions (one page at least, 2^30 positions at most)' % (W, pages.page_size))
+    row, one = t.stride()
+    if W > 1 and one != 1:
+        t = t.contiguous()
+        row = W
+    return t, row, W
 
 
 def _kv_aligned(t):
-    if t.stride(3) != 1 or t.data_ptr() & 15:
-        return False
     n = 16 // t.element_size() - 1
-    return not (t.stride(0) & n or t.stride(1) & n or t.stride(2) & n)
+    a, b, c, d = t.stride()
+    return d == 1 and not ((a | b | c) & n or t.data_ptr() & 15)
 
 
 def _kv_rows(t, name, pages, heads):
-    """(B, T, heads, head_dim) rows of an activation type: any strides; copied where a row is not dense or not 16-byte aligned"""
+    """(B, T, heads, head_dim) rows of an activation type, any strides; copied where a row is not dense or not 16-byte aligned"""
     if not isinstance(t, torch.Tensor) or t.dim() != 4:
         raise RuntimeError('%s must be a (sequences, tokens, heads, head_dim) tensor' % name)
     if t.device != pages.device:
+        if not t.is_cuda:
+            raise RuntimeError('%s must live on a HIP device (got %s); the MI355X backend has no CPU path' % (name, t.device))
         raise RuntimeError('%s is on %s, the pool on %s' % (name, t.device, pages.device))
     if t.dtype not in _KV_ROW_TYPES:
         raise RuntimeError('%s must be float32, bfloat16 or float16 (got %s)' % (name, t.dtype))
-    if t.shape[3] != pages.head_dim or (t.shape[2] != heads if heads else t.shape[2] < 1 or t.shape[2] % pages.heads):
-        raise RuntimeError('%s: %d heads of %d over a pool of %d heads of %d' % (name, t.shape[2], t.shape[3], pages.heads, pages.head_dim))
+    B, _, H, D = t.shape
+    if D != pages.head_dim or (H != heads if heads else H < 1 or H % pages.heads):
+        raise RuntimeError('%s: %d heads of %d over a pool of %d heads of %d' % (name, H, D, pages.heads, pages.head_dim))
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError('%s requires a gradient: the paged cache is forward only (call it under torch.no_grad())' % name)
-    if t.shape[0] > 65535:
-        raise RuntimeError('%s: %d sequences (at most 65535)' % (name, t.shape[0]))
+    if B > 65535:
+        raise RuntimeError('%s: %d sequences (at most 65535)' % (name, B))
     if _kv_aligned(t):
         return t
     t = t.contiguous()
@@ -1718,15 +1727,15 @@ def kv_append(pages, k, v, table, lens, new_lens=None):
     if k.stride() != v.stride():
         k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
     B, T = k.shape[:2]
-    table = _kv_table(table, pages, B)
-    lens = _kv_ints(lens, 'lens', pages, (B,))
-    new_lens = _kv_ints(new_lens, 'new_lens', pages, (B,)) if new_lens is not None else None
+    table, row, width = _kv_table(table, pages, B)
+    lens = _kv_ints(lens, 'lens', pages, B)
+    new_lens = _kv_ints(new_lens, 'new_lens', pages, B) if new_lens is not None else None
     if B == 0 or T == 0:
         return pages
     sb, st, sh, _ = k.stride()
     with _on(pages.device):
-        _lib.call('pvsg_kv_append', pages._struct, k.data_ptr(), v.data_ptr(), _KV_ROW_TYPES[k.dtype], sb, st, sh, table.data_ptr(),
-                  table.stride(0), table.shape[1], lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, B, T,
+        _lib.call('pvsg_kv_append', pages._struct, k.data_ptr(), v.data_ptr(), _KV_ROW_TYPES[k.dtype], sb, st, sh, table.data_ptr(), row,
+                  width, lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, B, T,
                   _stream_ptr())
     return pages
 
@@ -1739,17 +1748,17 @@ def kv_read(pages, table, lens, length, start=0, dtype=torch.float32):
     length, start = int(length), int(start)
     if length < 0 or start < 0 or start + length >= 1 << 31:
         raise RuntimeError('kv_read: positions %d .. %d + %d' % (start, start, length))
-    table = _kv_table(table, pages, None)
+    table, row, width = _kv_table(table, pages, None)
     B = table.shape[0]
     if B > 65535:
         raise RuntimeError('kv_read: %d sequences (at most 65535)' % B)
-    lens = _kv_ints(lens, 'lens', pages, (B,))
+    lens = _kv_ints(lens, 'lens', pages, B)
     out = [torch.empty((B, length, pages.heads, pages.head_dim), device=pages.device, dtype=dtype) for _ in range(2)]
     if B == 0 or length == 0:
         return tuple(out)
     with _on(pages.device):
-        _lib.call('pvsg_kv_read', pages._struct, out[0].data_ptr(), out[1].data_ptr(), _KV_ROW_TYPES[dtype], table.data_ptr(),
-                  table.stride(0), table.shape[1], lens.data_ptr(), B, start, length, _stream_ptr())
+        _lib.call('pvsg_kv_read', pages._struct, out[0].data_ptr(), out[1].data_ptr(), _KV_ROW_TYPES[dtype], table.data_ptr(), row,
+                  width, lens.data_ptr(), B, start, length, _stream_ptr())
     return tuple(out)
 
 
@@ -1772,9 +1781,9 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
         raise RuntimeError('paged_attention: %d query heads over %d key heads' % (HQ, pages.heads))
     if q.dtype != pages.dtype and q.dtype != torch.float32 and pages.dtype not in _KV_SCALED:
         raise RuntimeError('paged_attention: %s rows over a %s pool' % (q.dtype, pages.dtype))
-    table = _kv_table(table, pages, B)
-    lens = _kv_ints(lens, 'lens', pages, (B,))
-    new_lens = _kv_ints(new_lens, 'new_lens', pages, (B,)) if new_lens is not None else None
+    table, table_row, width = _kv_table(table, pages, B)
+    lens = _kv_ints(lens, 'lens', pages, B)
+    new_lens = _kv_ints(new_lens, 'new_lens', pages, B) if new_lens is not None else None
     mask, ms, mw = None, 0, 0
     if key_padding_mask is not None:
         mask = key_padding_mask
@@ -1784,7 +1793,7 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
             mask = mask.contiguous()
         ms, mw = mask.stride(0), mask.shape[1]
     if out is None:
-        out = torch.empty((B, T, HQ, D), device=q.device, dtype=q.dtype)
+        out = q.new_empty((B, T, HQ, D))
     elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or \
             out.data_ptr() & 15 or out.requires_grad:
         raise RuntimeError('paged_attention: out must be a contiguous, 16-byte aligned %s tensor of shape %s on %s' % (q.dtype, tuple(q.shape), q.device))
@@ -1792,12 +1801,12 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
         return out.zero_()
     if B == 0 or T == 0:
         return out
-    width, row, longest = table.shape[1], _KV_ROW_TYPES[q.dtype], 0 if max_len is None else max(1, int(max_len))
+    row, longest = _KV_ROW_TYPES[q.dtype], 0 if max_len is None else max(1, int(max_len))
     nbytes = _lib.load().pvsg_paged_attention_workspace_bytes(pages._struct, B, T, HQ, row, width, longest)
-    work = torch.empty((nbytes,), device=q.device, dtype=torch.uint8) if nbytes else None
+    work = lens.new_empty(nbytes // 4) if nbytes else None
     sb, st, sh, _ = q.stride()
     with _on(pages.device):
-        _lib.call('pvsg_paged_attention', pages._struct, q.data_ptr(), sb, st, sh, out.data_ptr(), row, table.data_ptr(), table.stride(0), width,
+        _lib.call('pvsg_paged_attention', pages._struct, q.data_ptr(), sb, st, sh, out.data_ptr(), row, table.data_ptr(), table_row, width,
                   lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, mask.data_ptr() if mask is not None else None,
                   ms, mw, B, T, HQ, D ** -0.5 if scale is None else float(scale), 1 if causal else 0, longest,
                   work.data_ptr() if work is not None else None, _stream_ptr())
