@@ -686,13 +686,17 @@ int pvsg_kv_read(const pvsg_kv_pages* pages, void* k_out, void* v_out, int out_t
  * (B, padding_width) rows padding_stride apart, nonzero = ignored) only p < padding_width with a zero there.  softmax(scale * q.k) v in f32, rounded
  * once; a row that sees nothing, or past n_b, is zero.  What a row does not see does not reach it, NaN and infinities included.
  * max_len: the longest cache to plan for (0: what the table holds); longer ones are computed all the same.
- * workspace: pvsg_paged_attention_workspace_bytes of the same arguments (0: none), 16-byte aligned, no initialisation. */
+ * workspace: pvsg_paged_attention_workspace_bytes of the same arguments (0: none), 16-byte aligned, no initialisation.
+ * counters: NULL, or PVSG_PAGED_ATTENTION_COUNTERS words that were zero before the first call that was given them and that no two calls
+ * in flight share; every call leaves them zero.  With them the parts of a split row are joined in the same launch, without in a second one. */
+#define PVSG_PAGED_ATTENTION_COUNTERS 1024
 long long pvsg_paged_attention_workspace_bytes(const pvsg_kv_pages* pages, int B, int T, int q_heads, int row_type, int table_width,
                                                long long max_len);
 int pvsg_paged_attention(const pvsg_kv_pages* pages, const void* q, long long q_seq_stride, long long q_token_stride,
                          long long q_head_stride, void* out, int row_type, const int* table, long long table_stride, int table_width,
                          const int* lens, const int* new_lens, const uint8_t* padding, long long padding_stride, int padding_width,
-                         int B, int T, int q_heads, float scale, int causal, long long max_len, void* workspace, void* stream);
+                         int B, int T, int q_heads, float scale, int causal, long long max_len, void* workspace, uint32_t* counters,
+                         void* stream);
 
 #ifdef __cplusplus
 }

@@ -154,7 +154,7 @@ SIGNATURES = {
     'pvsg_kv_read': [ctypes.POINTER(KvPages), _c_f, _c_f, _i, _c_f, _ll, _i, _c_f, _i, _i, _i, _c_f],
     'pvsg_paged_attention_workspace_bytes': [ctypes.POINTER(KvPages), _i, _i, _i, _i, _i, _ll],
     'pvsg_paged_attention': [ctypes.POINTER(KvPages), _c_f, _ll, _ll, _ll, _c_f, _i, _c_f, _ll, _i, _c_f, _c_f, _c_f, _ll, _i, _i, _i,
-                             _i, _f, _i, _ll, _c_f, _c_f],
+                             _i, _f, _i, _ll, _c_f, _c_f, _c_f],
 }
 # entry points that return a value instead of a status code
 VALUE_RETURNING = ('pvsg_xattn_num_splits', 'pvsg_gemm_bf16x3_packed_elems', 'pvsg_gemm_f16x2_packed_elems',

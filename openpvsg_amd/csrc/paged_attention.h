@@ -43,6 +43,7 @@ struct PagedAttn {
   int B, T, q_heads, group, rows, row_groups, causal;
   int workgroups;                        // how many share the tiles; 0: one for each (sequence, key head, row group)
   int* part_of;                          // of each: the sequence, the key head and row group, and the last workgroup that it splits with
+  unsigned* arrived;                     // zeros, one for each: the last workgroup of a row joins its parts; null: a second kernel does
 };
 
 constexpr int PA_WAVES = 4;
@@ -125,6 +126,77 @@ __device__ __forceinline__ void pa_store_row4(unsigned char* out, long long at, 
   }
 }
 
+// A part's values between workgroups.  FRESH: written in this launch, so they are read past the caches that other workgroups' stores do
+// not reach.
+template <bool FRESH>
+__device__ __forceinline__ float2 pa_part2(const float* p) {
+  if constexpr (FRESH) {
+    const unsigned long long u = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__builtin_bit_cast(float, (unsigned)u), __builtin_bit_cast(float, (unsigned)(u >> 32)));
+  } else {
+    return *reinterpret_cast<const float2*>(p);
+  }
+}
+__device__ __forceinline__ void pa_put2(float* p, float x, float y) {
+  const unsigned long long u = __builtin_bit_cast(unsigned, x) | (unsigned long long)__builtin_bit_cast(unsigned, y) << 32;
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(p), u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// The parts that the stretches of workgroups first .. first + n - 1 left of the `tile_rows` rows at row0 of key head h: joined and written.
+// dim / 4 threads across a row; of the groups of so many threads, `share` take one row's parts between them, so that few rows of
+// many parts are read at once as well.  The parts come in the stretches' order, whoever joins them.
+template <int RT, bool FRESH, class A>
+__device__ void pa_join(A& a, int b, int h, int row0, int tile_rows, int first, int n, int fresh, float (*s_o)[4], float* s_m, float* s_l) {
+  const int rows = min(tile_rows, a.rows - row0);
+  const int D = a.p.dim, d4 = D / 4, groups = 256 / d4, x = threadIdx.x % d4, y = threadIdx.x / d4;
+  const int share = max(1, min(groups / rows, n / 2)), at_once = groups / share;
+  for (int r0 = 0; r0 < rows; r0 += at_once) {
+    const int r = r0 + y / share, k0 = y % share;
+    const bool mine = y < at_once * share && r < rows;
+    // part k: what the first stretch left at its end, then what each later one left at its beginning
+    float top = -INFINITY, sum = 0.f, o[4] = {};
+    if (mine) {
+#pragma unroll 4
+      for (int k = k0; k < n; k += share) {
+        const long long slot = (long long)(2 * (first + k) + (k == 0 ? 1 : 0)) * tile_rows + r;
+        const float2 p = pa_part2<FRESH>(a.part_ml + 2 * slot);
+        const float2 v = pa_part2<FRESH>(a.part_o + slot * D + 4 * x), u = pa_part2<FRESH>(a.part_o + slot * D + 4 * x + 2);
+        const float up = fmaxf(top, p.x), ref = up == -INFINITY ? 0.f : up;
+        const float keep = __builtin_amdgcn_exp2f(top - ref), w = __builtin_amdgcn_exp2f(p.x - ref);
+        sum = sum * keep + w * p.y;
+        o[0] = o[0] * keep + w * v.x, o[1] = o[1] * keep + w * v.y, o[2] = o[2] * keep + w * u.x, o[3] = o[3] * keep + w * u.y;
+        top = up;
+      }
+    }
+    if (share > 1) {
+      __syncthreads();
+      st4(s_o[threadIdx.x], make_float4(o[0], o[1], o[2], o[3]));
+      s_m[threadIdx.x] = top, s_l[threadIdx.x] = sum;
+      __syncthreads();
+      if (mine && k0 == 0) {
+        float up = top;
+        for (int s = 1; s < share; ++s) up = fmaxf(up, s_m[threadIdx.x + s * d4]);
+        const float ref = up == -INFINITY ? 0.f : up, keep = __builtin_amdgcn_exp2f(top - ref);
+        sum *= keep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] *= keep;
+        for (int s = 1; s < share; ++s) {
+          const float w = __builtin_amdgcn_exp2f(s_m[threadIdx.x + s * d4] - ref);
+          const float4 v = ld4(s_o[threadIdx.x + s * d4]);
+          sum += w * s_l[threadIdx.x + s * d4];
+          o[0] += w * v.x, o[1] += w * v.y, o[2] += w * v.z, o[3] += w * v.w;
+        }
+      }
+    }
+    if (mine && k0 == 0) {
+      const int t = (row0 + r) / a.group;
+      const bool some = t < fresh && !(sum == 0.f);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = some ? o[i] / sum : 0.f;
+      pa_store_row4<RT>(a.out, (((long long)b * a.T + t) * a.q_heads + h * a.group + (row0 + r) % a.group) * D + 4 * x, o);
+    }
+  }
+}
+
 // Rows r0 .. r1-1 of one (sequence, key head) over the keys lo .. hi-1, by plain sums, a key at a time: the fallback for values that are
 // not finite.  buf: 3 * 256 floats of LDS; part_o / part_ml: where a part goes, null for the result itself.
 template <int RT, int CT>
@@ -195,8 +267,8 @@ __device__ void pa_rows_alone(PagedAttnArgs& a, int b, int h, int lo, int hi, in
     const long long row = ((long long)b * a.T + t) * a.q_heads + hq;
     if (tid < D) {
       if (part_o) {
-        part_o[(r - r0) * D + tid] = o;
-        if (tid == 0) *reinterpret_cast<float2*>(part_ml + (r - r0) * 2) = make_float2(top, sum);
+        __hip_atomic_store(&part_o[(r - r0) * D + tid], o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (tid == 0) pa_put2(part_ml + (r - r0) * 2, top, sum);
       } else {
         const float y = sum == 0.f ? 0.f : o / sum;
         if constexpr (RT == KV_F32) reinterpret_cast<float*>(a.out)[row * D + tid] = y;
@@ -244,17 +316,22 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
   // entries that stand for what a part costs beside its tiles, then its tiles.  hr: the first one of sequence b that the stretch
   // meets, `at` the entry of it where the stretch begins, `left` how many entries it has.
   int b, hr, at, left, len;
-  unsigned share = 0, more = 0;                                     // workgroup i takes `share` entries, and one more if i < more
+  unsigned share = 0, more = 0, first = 0;                          // workgroup i takes `share` entries, and one more if i < more; the next of this one's
   const int each = args->p.heads * args->row_groups;
   if (PagedAttnArgs& a = *args; a.workgroups == 0) {
     b = blockIdx.x / each, hr = blockIdx.x % each, at = 0;
     len = pa_const(a.lens)[b];
     left = INT_MAX;
   } else {
-    // every wave scans the lengths by itself: 64 lanes, `per` sequences each
+    // every wave scans the lengths by itself: 64 lanes, `per` sequences each, the first four of them in registers
     const int lane = threadIdx.x & 63, per = (a.B + 63) / 64, b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B), capacity = a.width << a.page_shift;
+    int lens[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) lens[k] = b0 + k < b1 ? a.lens[b0 + k] : 0;
     unsigned mine = 0;
-    for (int i = b0; i < b1; ++i) mine += PA_PART + tiles_of(a.lens[i], capacity);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) mine += b0 + k < b1 ? PA_PART + tiles_of(lens[k], capacity) : 0;
+    for (int i = b0 + 4; i < b1; ++i) mine += PA_PART + tiles_of(a.lens[i], capacity);
     mine *= each;
     unsigned upto = mine;
 #pragma unroll
@@ -265,23 +342,27 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
     const unsigned total = __builtin_amdgcn_readlane(upto, 63);
     const unsigned used = min((unsigned)a.workgroups, (total + PA_PART + PA_GRAIN - 1) / (PA_PART + PA_GRAIN));
     share = total / used, more = total - share * used;
-    const unsigned first = blockIdx.x * share + min(blockIdx.x, more);
-    if (threadIdx.x == 0) a.part_of[3 * blockIdx.x] = -1;
+    first = blockIdx.x * share + min(blockIdx.x, more);
+    if (!a.arrived && threadIdx.x == 0) a.part_of[3 * blockIdx.x] = -1;
     if (blockIdx.x >= used) return;
     left = share + (blockIdx.x < more ? 1 : 0);
     const int whose = __builtin_ctzll(__ballot(first < upto));      // the lane whose sequences the stretch begins in
     unsigned before = upto - mine;
-    b = b0;
-    if (per > 1) {
-      for (; b < b1 - 1; ++b) {
-        const unsigned n = (PA_PART + tiles_of(a.lens[b], capacity)) * each;
-        if (first < before + n) break;
-        before += n;
-      }
+    b = b0, len = lens[0];
+    bool found = false;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const unsigned n = (PA_PART + tiles_of(lens[k], capacity)) * each;
+      found |= b0 + k >= b1 - 1 || first < before + n;
+      if (!found) before += n, b = b0 + k + 1, len = lens[k + 1];
     }
-    b = __builtin_amdgcn_readlane(b, whose);
+    while (!found && b < b1 - 1) {
+      const unsigned n = (PA_PART + tiles_of(len, capacity)) * each;
+      if (first < before + n) break;
+      before += n, len = a.lens[++b];
+    }
+    b = __builtin_amdgcn_readlane(b, whose), len = __builtin_amdgcn_readlane(len, whose);
     const unsigned inside = first - __builtin_amdgcn_readlane(before, whose);
-    len = pa_const(a.lens)[b];
     const unsigned n = PA_PART + tiles_of(len, capacity);
     hr = inside / n, at = inside - hr * n;
   }
@@ -295,52 +376,51 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
     const int D = a.p.dim, page_mask = a.p.page_size - 1, capacity = a.width << a.page_shift;
     if (next_b) len = pa_const(a.lens)[b];
     const int tiles = tiles_of(len, capacity);
-    int tile0 = 0, tile1 = tiles;
+    int tile0 = 0, tile1 = tiles, first_wg = 0, last_wg = 0;          // workgroups that have the first and the last of the tiles
     if (a.workgroups) {
       const int end = min(PA_PART + tiles, at + left);
       tile0 = max(at - PA_PART, 0), tile1 = max(end - PA_PART, 0);
-      left -= end - at;
+      const unsigned from = first - at;                             // where the row begins in the list
+      left -= end - at, first += end - at;
       if (tile0 == tile1) continue;
+      if (tile0 != 0 || tile1 != tiles) {
+        auto holder = [&](unsigned entry) { return entry < more * (share + 1) ? entry / (share + 1) : more + (entry - more * (share + 1)) / share; };
+        first_wg = holder(from + PA_PART), last_wg = holder(from + PA_PART + tiles - 1);
+      }
     } else {
       left = 0;
     }
-    const bool whole_row = tile0 == 0 && tile1 == tiles;
     float *part_o = nullptr, *part_ml = nullptr;
-    if (!whole_row) {
+    if (tile0 != 0 || tile1 != tiles) {
       // a stretch has one part at most that begins inside a row's tiles and one that only ends inside
       const int slot = 2 * blockIdx.x + (tile0 == 0 ? 1 : 0);
       part_o = a.part_o + (long long)slot * (16 * NT) * D;
       part_ml = a.part_ml + (long long)slot * (16 * NT) * 2;
-      if (tile0 == 0 && tid == 0) {
-        // the workgroup that has the last tile: this stretch ends inside, so that one lies tiles - tile1 entries behind it
-        const unsigned end = (blockIdx.x + 1) * share + min(blockIdx.x + 1, more) + (tiles - tile1) - 1;
-        a.part_of[3 * blockIdx.x] = b, a.part_of[3 * blockIdx.x + 1] = hr;
-        a.part_of[3 * blockIdx.x + 2] = end < more * (share + 1) ? end / (share + 1) : more + (end - more * (share + 1)) / share;
-      }
+      if (!a.arrived && tile0 == 0 && tid == 0) a.part_of[3 * blockIdx.x] = b, a.part_of[3 * blockIdx.x + 1] = hr, a.part_of[3 * blockIdx.x + 2] = last_wg;
     }
     const int h = hr / a.row_groups, row0 = hr % a.row_groups * (16 * NT);
-    const KvSpan span = kv_span_of(len, a.new_lens ? pa_const(a.new_lens)[b] : a.T, a.T, capacity);
-    const int past = span.len - span.fresh;
-    // what the first and the last real row of this group see
-    const int t_lo = row0 / a.group, t_hi = min((min(row0 + 16 * NT, a.rows) - 1) / a.group, span.fresh - 1);
-    const int most = min(t_lo < span.fresh ? (a.causal ? min(past + t_hi + 1, span.there) : span.there) : 0, (int)min((long long)tile1 * TILE, 1ll << 30));
-    const int least = a.causal ? min(past + t_lo + 1, span.there) : span.there;
+
+    // what depends on the length alone is asked for first: the page ids of the first keys, two a thread at most
+    const int there = min(max(len, 0), capacity), key1 = (int)min((long long)tile1 * TILE, (long long)there);
+    auto pages_of = [&](int c0) { return c0 < key1 ? ((min(c0 + PA_CHUNK, key1) - 1) >> a.page_shift) - (c0 >> a.page_shift) + 1 : 0; };
+    auto page_at = [&](int c0, int i) { return a.table[(long long)b * a.table_stride + (c0 >> a.page_shift) + i]; };
+    constexpr int PAGES = PA_CHUNK / 8 / (64 * PA_WAVES);
+    int page_id[PAGES];
+#pragma unroll
+    for (int i = 0; i < PAGES; ++i) page_id[i] = tid + i * 64 * PA_WAVES < pages_of(tile0 * TILE) ? page_at(tile0 * TILE, tid + i * 64 * PA_WAVES) : 0;
 
     // query rows, in the operand layout
     unsigned qf[NT][QN * (M16 ? 4 * QL : 1)];
-    int lim[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int r = row0 + nt * 16 + m, t = r / a.group, j = r % a.group;
-      const bool real = r < a.rows && t < span.fresh;
-      lim[nt] = !real ? most : a.causal ? min(past + t + 1, span.there) : span.there;
       const unsigned char* qr = a.q + b * a.q_seq + t * a.q_token + (long long)(h * a.group + j) * a.q_head;
       constexpr int STEP = M16 ? 8 : 4;
 #pragma unroll
       for (int i = 0; i < DP / 4 / STEP; ++i) {
         const int d = (i * STEP / KC) * 4 * KC + KC * g + i * STEP % KC;
         unsigned w[STEP * RB / 4] = {};
-        if (real && d < D) {
+        if (r < a.rows && d < D) {
           kv_load<16>(w, qr + d * RB);
           if constexpr (STEP * RB == 32) kv_load<16>(w + 4, qr + d * RB + 16);
         }
@@ -358,10 +438,20 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
       }
     }
 
+    const KvSpan span = kv_span_of(len, a.new_lens ? pa_const(a.new_lens)[b] : a.T, a.T, capacity);
+    const int past = span.len - span.fresh;
+    if (len > capacity && tid == 0) kv_fault(a.p.faults, 4);
+    // what the first and the last real row of this group see, and each of this lane's
+    const int t_lo = row0 / a.group, t_hi = min((min(row0 + 16 * NT, a.rows) - 1) / a.group, span.fresh - 1);
+    const int most = min(t_lo < span.fresh ? (a.causal ? past + t_hi + 1 : there) : 0, key1);
+    const int least = a.causal ? min(past + t_lo + 1, there) : there;
+    int lim[NT];
     f32x4 acc[NT][VE];
     float mrow[NT], lrow[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      const int r = row0 + nt * 16 + m, t = r / a.group;
+      lim[nt] = r >= a.rows || t >= span.fresh ? most : a.causal ? min(past + t + 1, there) : there;
       mrow[nt] = -INFINITY, lrow[nt] = 0.f;
 #pragma unroll
       for (int e = 0; e < VE; ++e) acc[nt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -377,15 +467,17 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
 
     for (int c0 = tile0 * TILE; c0 < most; c0 += PA_CHUNK) {
       const int c1 = min(c0 + PA_CHUNK, most);
-      const int first_page = c0 >> a.page_shift;
-      __syncthreads();                                                // the previous chunk's pages have been read
-      for (int i = tid; i <= ((c1 - 1) >> a.page_shift) - first_page; i += 64 * PA_WAVES) {
-        int page = a.table[(long long)b * a.table_stride + first_page + i];
-        if ((unsigned)page >= (unsigned)a.p.num_pages) {
-          page = -1;
-          kv_fault(a.p.faults, 4);
-        }
-        s_page[i] = page;
+      const int first_page = c0 >> a.page_shift, pages = pages_of(c0);
+      if (c0 > tile0 * TILE) {
+        __syncthreads();                                              // the last keys' pages have been read
+#pragma unroll
+        for (int i = 0; i < PAGES; ++i) page_id[i] = tid + i * 64 * PA_WAVES < pages ? page_at(c0, tid + i * 64 * PA_WAVES) : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < PAGES; ++i) {
+        const bool bad = (unsigned)page_id[i] >= (unsigned)a.p.num_pages;
+        if (bad) kv_fault(a.p.faults, 4);
+        if (tid + i * 64 * PA_WAVES < pages) s_page[tid + i * 64 * PA_WAVES] = bad ? -1 : page_id[i];
       }
       if constexpr (PADDED) {
         for (int i = tid; i < c1 - c0; i += 64 * PA_WAVES) {
@@ -637,8 +729,9 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
           const long long row = ((long long)b * a.T + t) * a.q_heads + h * a.group + r % a.group;
           off |= t < span.fresh && !(__builtin_fabsf(o[0]) + __builtin_fabsf(o[1]) + __builtin_fabsf(o[2]) + __builtin_fabsf(o[3]) < INFINITY);
           if (part_o) {
-            st4(part_o + (nt * 16 + ml) * D + d, make_float4(o[0], o[1], o[2], o[3]));
-            if (d == 0) *reinterpret_cast<float2*>(part_ml + (nt * 16 + ml) * 2) = make_float2(top, sum);
+            pa_put2(part_o + (nt * 16 + ml) * D + d, o[0], o[1]);
+            pa_put2(part_o + (nt * 16 + ml) * D + d + 2, o[2], o[3]);
+            if (d == 0) pa_put2(part_ml + (nt * 16 + ml) * 2, top, sum);
           } else {
             const bool some = t < span.fresh && !(sum == 0.f);
 #pragma unroll
@@ -651,8 +744,32 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
     // What a row does not see must not reach it, but 0 * infinity and 0 * NaN do in a matrix product over shared values, and an
     // infinite value meets the rest of its P, which may be 0 or negative.  So where a result is not finite, the rows are
     // computed again, each from what it sees alone.  (The barrier also parts these rows' LDS from the next ones'.)
-    if (__syncthreads_or(off))
+    if (__syncthreads_or(off)) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // what is stored above does not land on top of it
+      __syncthreads();
       pa_rows_alone<RT, CT>(a, b, h, tile0 * TILE, most, row0, min(row0 + 16 * NT, a.rows), span, part_o, part_ml, &s_o[0][0][0]);
+    }
+    if (a.arrived && part_o) {
+      // The last of a row's workgroups joins its parts.  Parts are stored through the caches that do not reach other workgroups, and
+      // every store is complete before this one counts; a release at device scope would write back everything those caches hold
+      // (measured: microseconds).  The counter is zero again for the next launch.
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (tid == 0) {
+        const unsigned n = last_wg - first_wg + 1;
+        const bool last = __hip_atomic_fetch_add(&a.arrived[first_wg], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+        if (last) __hip_atomic_store(&a.arrived[first_wg], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        s_page[0] = last;
+      }
+      __syncthreads();
+      const bool last = s_page[0] != 0;
+      __syncthreads();
+      if (last) {
+        float* buf = &s_o[0][0][0];
+        pa_join<RT, true>(a, b, h, row0, 16 * NT, first_wg, last_wg - first_wg + 1, span.fresh, reinterpret_cast<float(*)[4]>(buf), buf + 1024, buf + 1280);
+        __syncthreads();
+      }
+    }
   }
 }
 

@@ -3,66 +3,17 @@
 
 namespace pvsg {
 
-// The join: workgroup i looks at the part that workgroup i of the first kernel left of a (sequence, key head, row group) that ends in a
-// later stretch, and adds the parts of the stretches up to that one.  dim / 4 threads across a row; of the groups of so many
-// threads, `share` take one row's parts between them, so that few rows of many parts are read at once as well.
+// The join as a kernel of its own: workgroup i looks at the part that workgroup i of the first kernel left of a row that ends in a later
+// stretch.
 template <int RT>
 __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAttn a, int tile_rows) {
+  __shared__ __align__(16) float s_o[256][4];
+  __shared__ float s_m[256], s_l[256];
   const int first = blockIdx.x, b = a.part_of[3 * first];
   if (b < 0) return;
   const int hr = a.part_of[3 * first + 1], n = a.part_of[3 * first + 2] - first + 1;
   const KvSpan span = kv_span(a.lens, a.new_lens, b, a.T, a.width << a.page_shift);
-  const int h = hr / a.row_groups, row0 = hr % a.row_groups * tile_rows, rows = min(tile_rows, a.rows - row0);
-  const int D = a.p.dim, d4 = D / 4, groups = 256 / d4, x = threadIdx.x % d4, y = threadIdx.x / d4;
-  const int share = max(1, min(groups / rows, n / 2)), at_once = groups / share;
-  __shared__ __align__(16) float s_o[256][4];
-  __shared__ float s_m[256], s_l[256];
-  for (int r0 = 0; r0 < rows; r0 += at_once) {
-    const int r = r0 + y / share, k0 = y % share;
-    const bool mine = y < at_once * share && r < rows;
-    // part k: what the first stretch left at its end, then what each later one left at its beginning
-    float top = -INFINITY, sum = 0.f, o[4] = {};
-    if (mine) {
-#pragma unroll 4
-      for (int k = k0; k < n; k += share) {
-        const long long slot = (long long)(2 * (first + k) + (k == 0 ? 1 : 0)) * tile_rows + r;
-        const float2 p = *reinterpret_cast<const float2*>(a.part_ml + 2 * slot);
-        const float4 v = ld4(a.part_o + slot * D + 4 * x);
-        const float up = fmaxf(top, p.x), ref = up == -INFINITY ? 0.f : up;
-        const float keep = __builtin_amdgcn_exp2f(top - ref), w = __builtin_amdgcn_exp2f(p.x - ref);
-        sum = sum * keep + w * p.y;
-        o[0] = o[0] * keep + w * v.x, o[1] = o[1] * keep + w * v.y, o[2] = o[2] * keep + w * v.z, o[3] = o[3] * keep + w * v.w;
-        top = up;
-      }
-    }
-    if (share > 1) {
-      __syncthreads();
-      st4(s_o[threadIdx.x], make_float4(o[0], o[1], o[2], o[3]));
-      s_m[threadIdx.x] = top, s_l[threadIdx.x] = sum;
-      __syncthreads();
-      if (mine && k0 == 0) {
-        float up = top;
-        for (int s = 1; s < share; ++s) up = fmaxf(up, s_m[threadIdx.x + s * d4]);
-        const float ref = up == -INFINITY ? 0.f : up, keep = __builtin_amdgcn_exp2f(top - ref);
-        sum *= keep;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] *= keep;
-        for (int s = 1; s < share; ++s) {
-          const float w = __builtin_amdgcn_exp2f(s_m[threadIdx.x + s * d4] - ref);
-          const float4 v = ld4(s_o[threadIdx.x + s * d4]);
-          sum += w * s_l[threadIdx.x + s * d4];
-          o[0] += w * v.x, o[1] += w * v.y, o[2] += w * v.z, o[3] += w * v.w;
-        }
-      }
-    }
-    if (mine && k0 == 0) {
-      const int t = (row0 + r) / a.group;
-      const bool some = t < span.fresh && !(sum == 0.f);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = some ? o[i] / sum : 0.f;
-      pa_store_row4<RT>(a.out, (((long long)b * a.T + t) * a.q_heads + h * a.group + (row0 + r) % a.group) * D + 4 * x, o);
-    }
-  }
+  pa_join<RT, false>(a, b, hr / a.row_groups, hr % a.row_groups * tile_rows, tile_rows, first, n, span.fresh, s_o, s_m, s_l);
 }
 
 // caches of up to so many tiles are not split: each has a workgroup of its own
@@ -108,7 +59,7 @@ extern "C" long long pvsg_paged_attention_workspace_bytes(const pvsg_kv_pages* p
 extern "C" int pvsg_paged_attention(const pvsg_kv_pages* pages, const void* q, long long q_seq_stride, long long q_token_stride,
                                     long long q_head_stride, void* out, int row_type, const int* table, long long table_stride, int table_width,
                                     const int* lens, const int* new_lens, const uint8_t* padding, long long padding_stride, int padding_width,
-                                    int B, int T, int q_heads, float scale, int causal, long long max_len, void* workspace, void* stream) {
+                                    int B, int T, int q_heads, float scale, int causal, long long max_len, void* workspace, uint32_t* counters, void* stream) {
   using namespace pvsg;
   if (const int rc = kv_check_pages("pvsg_paged_attention", pages, table, table_stride, table_width, lens, B)) return rc;
   PVSG_REQUIRE(q && out, "pvsg_paged_attention: null pointer");
@@ -139,11 +90,12 @@ extern "C" int pvsg_paged_attention(const pvsg_kv_pages* pages, const void* q, l
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + s.part_o;
     a.part_of = reinterpret_cast<int*>(a.part_ml + s.part_ml);
+    a.arrived = counters;
   }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   (row_type == KV_F32 ? pa_run_f32 : row_type == KV_BF16 ? pa_run_bf16 : pa_run_f16)(a, s.tiles, (unsigned)(s.workgroups ? s.workgroups : s.units), st);
   PVSG_LAUNCH_CHECK("pvsg_paged_attention");
-  if (s.workgroups > 1) {
+  if (s.workgroups > 1 && !counters) {
     const dim3 grid((unsigned)(s.workgroups - 1));
     if (row_type == KV_F32) hipLaunchKernelGGL((paged_attention_join_kernel<KV_F32>), grid, dim3(256), 0, st, a, 16 * s.tiles);
     else if (row_type == KV_BF16) hipLaunchKernelGGL((paged_attention_join_kernel<KV_BF16>), grid, dim3(256), 0, st, a, 16 * s.tiles);

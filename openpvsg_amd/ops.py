@@ -1762,6 +1762,21 @@ def kv_read(pages, table, lens, length, start=0, dtype=torch.float32):
     return tuple(out)
 
 
+_attention_counters = {}
+
+
+def _paged_attention_counters(device, stream):
+    """Zeroed words by which the workgroups of a launch find out who joins a split row: one set for each stream, whose launches
+    follow each other and leave them zero.  None while a graph is captured: its replays may run beside anything, so a second
+    launch joins there."""
+    if torch.cuda.is_current_stream_capturing():
+        return None
+    t = _attention_counters.get((device, stream))
+    if t is None:
+        t = _attention_counters[device, stream] = torch.zeros(1024, dtype=torch.int32).to(torch.device('cuda', device))
+    return t.data_ptr()
+
+
 def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None, causal=True, scale=None, max_len=None, out=None):
     """Attention of new tokens over the cached keys and values: softmax(scale * q . k) v, in float32, rounded once to q's dtype.
 
@@ -1806,8 +1821,9 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
     work = lens.new_empty(nbytes // 4) if nbytes else None
     sb, st, sh, _ = q.stride()
     with _on(pages.device):
+        stream = _stream_ptr()
         _lib.call('pvsg_paged_attention', pages._struct, q.data_ptr(), sb, st, sh, out.data_ptr(), row, table.data_ptr(), table_row, width,
                   lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, mask.data_ptr() if mask is not None else None,
                   ms, mw, B, T, HQ, D ** -0.5 if scale is None else float(scale), 1 if causal else 0, longest,
-                  work.data_ptr() if work is not None else None, _stream_ptr())
+                  work.data_ptr() if work is not None else None, _paged_attention_counters(q.device.index, stream) if nbytes else None, stream)
     return out

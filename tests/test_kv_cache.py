@@ -149,7 +149,7 @@ def test_bad_pools_are_refused(hip_lib, bad):
     p, one = pages_struct(**bad), ctypes.c_void_p(4096)
     assert hip_lib.pvsg_kv_append(p, one, one, 0, 64, 64, 64, one, 2, 2, one, None, 1, 1, None) == 1
     assert hip_lib.pvsg_kv_read(p, one, one, 0, one, 2, 2, one, 1, 0, 4, None) == 1
-    assert hip_lib.pvsg_paged_attention(p, one, 64, 64, 64, one, 0, one, 2, 2, one, None, None, 0, 0, 1, 1, 4, 1.0, 1, 0, None, None) == 1
+    assert hip_lib.pvsg_paged_attention(p, one, 64, 64, 64, one, 0, one, 2, 2, one, None, None, 0, 0, 1, 1, 4, 1.0, 1, 0, None, None, None) == 1
     assert len(hip_lib.pvsg_last_error()) > 10
 
 
@@ -163,7 +163,7 @@ def test_bad_calls_are_refused(hip_lib):
         return hip_lib.pvsg_kv_read(p, out, one, kind, one, 2, 2, one, B, start, length, None)
 
     def attend(pool=p, q=one, out=one, row=0, T=1, HQ=4, width=2, work=None, st=(64, 64, 64), B=1):
-        return hip_lib.pvsg_paged_attention(pool, q, *st, out, row, one, width, width, one, None, None, 0, 0, B, T, HQ, 1.0, 1, 0, work, None)
+        return hip_lib.pvsg_paged_attention(pool, q, *st, out, row, one, width, width, one, None, None, 0, 0, B, T, HQ, 1.0, 1, 0, work, None, None)
 
     for rc in (append(k=None), append(row=3), append(st=(64, 64, 66)), append(table=None), append(width=0), append(width=1 << 27), append(lens=None),
                append(B=-1), append(B=70000), append(T=-1), append(k=ctypes.c_void_p(4100)),
