@@ -49,7 +49,7 @@ struct PagedAttn {
 constexpr int PA_WAVES = 4;
 constexpr int PA_CHUNK = 4096;           // keys whose pages are looked up at a time
 constexpr int PA_PART = 3;                // what a part costs beside its tiles, in tiles
-constexpr int PA_GRAIN = 2;               // tiles that a workgroup takes at least
+constexpr int PA_GRAIN = 1;               // tiles that a workgroup takes at least
 constexpr int PA_MAX_T = 32;
 
 // The kernel reads its arguments where the launch left them, again for each part of its work: held in scalar registers
