@@ -1,8 +1,9 @@
 // Writing a paged key/value pool (quantising on the way) and reading it back dense.
 //
 // Both are one pass over the rows and bound by memory: a row is 2 * dim elements in one type in, the same in another out, and
-// a scale.  A lane holds 8 elements of a row's K and of its V (16-byte accesses on the 16-bit side), so a row is next_pow2(dim/8)
-// lanes: 16 at dim 128, four rows to a wave, and the row's maximum needs log2 of that in lane exchanges and no LDS.
+// a scale.  A lane holds 8 elements of a row's K and of its V, so a row is next_pow2(dim/8) lanes: 16 at dim 128, four rows to a
+// wave, and the row's maximum needs log2 of that in lane exchanges and no LDS.  The 8 elements are one run, or where one side is f32
+// two runs of 4, a row's lanes apart: every access is then dense over the lanes.
 #include "kv_pages.h"
 
 namespace pvsg {
@@ -35,7 +36,7 @@ struct KvAppend {
   const int* table;
   long long table_stride;
   const int *lens, *new_lens;
-  int width, T, page_shift, lanes_shift;
+  int width, T, page_shift, lanes_shift, run_shift;
 };
 
 constexpr float KV_TINY = 1.17549435e-38f;           // 2^-126: keeps x / s finite where the row is all zeros or denormal
@@ -92,8 +93,28 @@ __device__ __forceinline__ void kv_encode8(const float* x, const KvScale& k, uns
   }
 }
 
+constexpr int kv_run(int row_type, int pool_type) { return row_type == KV_F32 || pool_type == KV_F32 ? 4 : 8; }
+
+// this lane's 8 elements of a row that starts at `row`, dim of them in all
+template <int TYPE, int RUN>
+__device__ __forceinline__ void kv_load_run(unsigned (&w)[kv_bytes(TYPE) * 2], const unsigned char* row, int sub, int lanes, int dim) {
+#pragma unroll
+  for (int i = 0; i < 8 / RUN; ++i) {
+    const int d = RUN * (sub + i * lanes);
+    if (d < dim) kv_load_once<RUN * kv_bytes(TYPE)>(&w[i * RUN * kv_bytes(TYPE) / 4], row + d * kv_bytes(TYPE));
+  }
+}
+template <int TYPE, int RUN, bool ONCE>
+__device__ __forceinline__ void kv_store_run(unsigned char* row, const unsigned (&w)[kv_bytes(TYPE) * 2], int sub, int lanes, int dim) {
+#pragma unroll
+  for (int i = 0; i < 8 / RUN; ++i) {
+    const int d = RUN * (sub + i * lanes);
+    if (d < dim) kv_store<RUN * kv_bytes(TYPE), ONCE>(row + d * kv_bytes(TYPE), &w[i * RUN * kv_bytes(TYPE) / 4]);
+  }
+}
+
 template <int RT, int CT>
-__device__ __forceinline__ void kv_append_row(const unsigned (&raw)[kv_bytes(RT) * 2], unsigned char* dst, float* scale, int lanes, bool live, bool lane0, bool in_dim) {
+__device__ __forceinline__ void kv_append_row(const unsigned (&raw)[kv_bytes(RT) * 2], unsigned char* dst, float* scale, int sub, int lanes, int dim, bool live) {
   float x[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = kv_elem<RT>(raw, i);
@@ -110,18 +131,11 @@ __device__ __forceinline__ void kv_append_row(const unsigned (&raw)[kv_bytes(RT)
     k.s = k.s < KV_TINY ? KV_TINY : k.s;               // a NaN stays
     k.y = 1.f / k.s;
     k.odd = __any(!(k.s < INFINITY));
-    if (live && lane0) *scale = k.s;
+    if (live && sub == 0) *scale = k.s;
   }
-  if (live && in_dim) {
-    unsigned w[kv_bytes(CT) * 2];
-    kv_encode8<CT>(x, k, w);
-    if constexpr (CT == KV_F32) {
-      kv_store<16>(dst, w);
-      kv_store<16>(dst + 16, w + 4);
-    } else {
-      kv_store<kv_bytes(CT) * 8>(dst, w);
-    }
-  }
+  unsigned w[kv_bytes(CT) * 2];
+  kv_encode8<CT>(x, k, w);
+  if (live) kv_store_run<CT, kv_run(RT, CT), false>(dst, w, sub, lanes, dim);
 }
 
 template <int RT, int CT>
@@ -130,7 +144,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppend a) {
   const int b = blockIdx.y;
   const int lanes = 1 << a.lanes_shift;
   const int sub = threadIdx.x & (lanes - 1);
-  const unsigned r = (blockIdx.x << (8 - a.lanes_shift)) + (threadIdx.x >> a.lanes_shift), t = r / a.p.heads, h = r % a.p.heads;
+  // runs of 2^run_shift tokens of one head, so that a workgroup's scales lie together: 4-byte pieces of one line from many
+  // workgroups, each behind another L2, cost as much as the codes (measured at 16 x 4096 rows into int8: 93 -> 86 us)
+  const unsigned r = (blockIdx.x << (8 - a.lanes_shift)) + (threadIdx.x >> a.lanes_shift), run = r >> a.run_shift;
+  const unsigned t = ((run / a.p.heads) << a.run_shift) + (r & ((1u << a.run_shift) - 1)), h = run % a.p.heads;
   const KvSpan span = kv_span(a.lens, a.new_lens, b, a.T, a.width << a.page_shift);
   bool live = (int)t < span.fresh;
   const int pos = live ? span.len - span.fresh + (int)t : 0;
@@ -143,22 +160,17 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppend a) {
       if (sub == 0) kv_fault(a.p.faults, 1);
     }
   }
-  const bool in_dim = 8 * sub < a.p.dim;
   unsigned kr[RB * 2] = {}, vr[RB * 2] = {};
-  if (live && in_dim) {
-    const long long src = b * a.seq_stride + (long long)t * a.token_stride + (long long)h * a.head_stride + sub * (8 * RB);
-    kv_load<16>(kr, a.k + src);
-    kv_load<16>(vr, a.v + src);
-    if constexpr (RB == 4) {
-      kv_load<16>(kr + 4, a.k + src + 16);
-      kv_load<16>(vr + 4, a.v + src + 16);
-    }
+  if (live) {
+    const long long src = b * a.seq_stride + (long long)t * a.token_stride + (long long)h * a.head_stride;
+    kv_load_run<RT, kv_run(RT, CT)>(kr, a.k + src, sub, lanes, a.p.dim);
+    kv_load_run<RT, kv_run(RT, CT)>(vr, a.v + src, sub, lanes, a.p.dim);
   }
   const int slot = pos & (a.p.page_size - 1);
-  const long long dst = ((long long)page * a.p.page_stride + (long long)h * a.p.head_stride + (long long)slot * a.p.slot_stride + 8 * sub) * CB;
+  const long long dst = ((long long)page * a.p.page_stride + (long long)h * a.p.head_stride + (long long)slot * a.p.slot_stride) * CB;
   const long long sc = (long long)page * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + slot;
-  kv_append_row<RT, CT>(kr, static_cast<unsigned char*>(a.p.k) + dst, a.p.k_scale + sc, lanes, live, sub == 0, in_dim);
-  kv_append_row<RT, CT>(vr, static_cast<unsigned char*>(a.p.v) + dst, a.p.v_scale + sc, lanes, live, sub == 0, in_dim);
+  kv_append_row<RT, CT>(kr, static_cast<unsigned char*>(a.p.k) + dst, a.p.k_scale + sc, sub, lanes, a.p.dim, live);
+  kv_append_row<RT, CT>(vr, static_cast<unsigned char*>(a.p.v) + dst, a.p.v_scale + sc, sub, lanes, a.p.dim, live);
 }
 
 struct KvRead {
@@ -172,11 +184,11 @@ struct KvRead {
 
 template <int RT, int CT>
 __global__ __launch_bounds__(256) void kv_read_kernel(const KvRead a) {
-  constexpr int RB = kv_bytes(RT), CB = kv_bytes(CT);
+  constexpr int RB = kv_bytes(RT), CB = kv_bytes(CT), RUN = kv_run(RT, CT);
   const int b = blockIdx.y;
-  const int sub = threadIdx.x & ((1 << a.lanes_shift) - 1);
+  const int lanes = 1 << a.lanes_shift, sub = threadIdx.x & (lanes - 1);
   const unsigned r = (blockIdx.x << (8 - a.lanes_shift)) + (threadIdx.x >> a.lanes_shift), t = r / a.p.heads, h = r % a.p.heads;
-  if ((int)t >= a.length || 8 * sub >= a.p.dim) return;
+  if ((int)t >= a.length) return;
   const KvSpan span = kv_span(a.lens, nullptr, b, 0, a.width << a.page_shift);
   const long long pos = a.start + (long long)t;
   unsigned kw[CB * 2] = {}, vw[CB * 2] = {};
@@ -185,14 +197,9 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvRead a) {
     const int page = pos < span.there ? a.table[(long long)b * a.table_stride + (pos >> a.page_shift)] : -1;
     if ((unsigned)page < (unsigned)a.p.num_pages) {
       const int slot = (int)pos & (a.p.page_size - 1);
-      const long long src = ((long long)page * a.p.page_stride + (long long)h * a.p.head_stride + (long long)slot * a.p.slot_stride + 8 * sub) * CB;
-      constexpr int N = CB == 4 ? 16 : CB * 8;
-      kv_load<N>(kw, static_cast<const unsigned char*>(a.p.k) + src);
-      kv_load<N>(vw, static_cast<const unsigned char*>(a.p.v) + src);
-      if constexpr (CB == 4) {
-        kv_load<16>(kw + 4, static_cast<const unsigned char*>(a.p.k) + src + 16);
-        kv_load<16>(vw + 4, static_cast<const unsigned char*>(a.p.v) + src + 16);
-      }
+      const long long src = ((long long)page * a.p.page_stride + (long long)h * a.p.head_stride + (long long)slot * a.p.slot_stride) * CB;
+      kv_load_run<CT, RUN>(kw, static_cast<const unsigned char*>(a.p.k) + src, sub, lanes, a.p.dim);
+      kv_load_run<CT, RUN>(vw, static_cast<const unsigned char*>(a.p.v) + src, sub, lanes, a.p.dim);
       if constexpr (kv_scaled(CT)) {
         const long long sc = (long long)page * a.p.scale_page_stride + (long long)h * a.p.scale_head_stride + slot;
         ks = a.p.k_scale[sc], vs = a.p.v_scale[sc];
@@ -201,7 +208,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvRead a) {
       kv_fault(a.p.faults, 2);
     }
   }
-  const long long dst = (((long long)b * a.length * a.p.heads + r) * a.p.dim + 8 * sub) * RB;
+  const long long dst = ((long long)b * a.length * a.p.heads + r) * a.p.dim * RB;
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const unsigned* w = which ? vw : kw;
@@ -213,9 +220,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(const KvRead a) {
     }
     unsigned o[RB * 2];
     kv_encode8<RT>(x, KvScale{1.f, 1.f, false}, o);
-    unsigned char* out = (which ? a.v : a.k) + dst;
-    kv_store<16>(out, o);
-    if constexpr (RB == 4) kv_store<16>(out + 16, o + 4);
+    kv_store_run<RT, RUN, true>((which ? a.v : a.k) + dst, o, sub, lanes, a.p.dim);
   }
 }
 
@@ -266,8 +271,9 @@ extern "C" int pvsg_kv_append(const pvsg_kv_pages* pages, const void* k, const v
   PVSG_REQUIRE(T >= 0, "pvsg_kv_append: %d tokens", T);
   if (B == 0 || T == 0) return PVSG_OK;
   KvAppend a{*pages, static_cast<const unsigned char*>(k), static_cast<const unsigned char*>(v), seq_stride * rb, token_stride * rb, head_stride * rb,
-             table, table_stride, lens, new_lens, table_width, T, kv_log2(pages->page_size), kv_log2(pages->dim / 8)};
-  const long long rows = (long long)T * pages->heads, blocks = ((rows << a.lanes_shift) + 255) / 256;
+             table, table_stride, lens, new_lens, table_width, T, kv_log2(pages->page_size), kv_log2(pages->dim / 8), 0};
+  while ((2 << a.run_shift) <= T && a.run_shift < 8 - a.lanes_shift) ++a.run_shift;
+  const long long rows = (((long long)T + (1 << a.run_shift) - 1) >> a.run_shift << a.run_shift) * pages->heads, blocks = ((rows << a.lanes_shift) + 255) / 256;
   PVSG_REQUIRE(rows < (1ll << 31) - 256, "pvsg_kv_append: %d tokens of %d heads are too many for one launch", T, pages->heads);
   kv_launch(row_type, a, dim3((unsigned)blocks, (unsigned)B), static_cast<hipStream_t>(stream));
   PVSG_LAUNCH_CHECK("pvsg_kv_append");
