@@ -16,8 +16,10 @@ __global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAt
   pa_join<RT, false>(a, b, hr / a.row_groups, hr % a.row_groups * tile_rows, tile_rows, first, n, span.fresh, s_o, s_m, s_l);
 }
 
-// caches of up to so many tiles are not split: each has a workgroup of its own
-constexpr int PA_SHORT = 4;
+// Caches of up to so many tiles are not split: each has a workgroup of its own.  Measured over 4 .. 800 (sequence, key head)s of bf16
+// heads of 128: at 700 positions (6 tiles) 11.0 - 37.8 us so and 13.5 - 42.8 us split and joined, at 1000 (8) 13.5 - 50 and 13.7 -
+// 53.7, at 1500 (12) 17.6 - 70 and 13.5 - 71: the wait for a tile's memory, 1.2 us, is paid once a tile.
+constexpr int PA_SHORT = 8;
 
 // 16-row tiles a wave carries: two where there are more rows than one tile holds and the accumulators of two fit
 static int pa_tiles(int rows, int dim, int row_type) { return rows > 16 && dim <= (row_type == KV_F32 ? 64 : 128) ? 2 : 1; }

@@ -1638,7 +1638,11 @@ class KVPages:
             raise RuntimeError('KVPages: page_size must be a power of two in [8, 65536], with at least one page and head (got %s)' % (tuple(k.shape),))
         if D < 16 or D > 256 or D % 16:
             raise RuntimeError('KVPages: head_dim must be a multiple of 16 up to 256 (got %d)' % D)
-        if sd != 1 or sp % unit or sh % unit or ss % unit or ss < D or (k.data_ptr() | v.data_ptr()) & 15:
+        extent, apart = D, True
+        for stride, n in sorted(((sp, P), (sh, H), (ss, S))):
+            if n > 1:
+                apart, extent = apart and stride >= extent, stride * (n - 1) + extent
+        if sd != 1 or sp % unit or sh % unit or ss % unit or not apart or (k.data_ptr() | v.data_ptr()) & 15:
             raise RuntimeError('KVPages: rows must be dense, distinct and 16-byte aligned (strides %s)' % (k.stride(),))
         scaled = k.dtype in _KV_SCALED
         if scaled != (k_scale is not None) or scaled != (v_scale is not None):
@@ -1722,6 +1726,8 @@ def kv_append(pages, k, v, table, lens, new_lens=None):
     back as NaN.  Pages that are appended to belong to one sequence.  Page ids out of the pool: skipped, see page_fault_check."""
     k = _kv_rows(k, 'k', pages, pages.heads)
     v = _kv_rows(v, 'v', pages, pages.heads)
+    if pages.k.data_ptr() == pages.v.data_ptr():
+        raise RuntimeError('kv_append: the pool\'s k and v are the same memory')
     if k.shape != v.shape or k.dtype != v.dtype:
         raise RuntimeError('kv_append: k %s %s and v %s %s differ' % (tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
     if k.stride() != v.stride():

@@ -459,6 +459,49 @@ def test_bad_page_ids_and_lengths_are_skipped_and_reported(hip_lib):
 
 
 @gpu
+def test_idle_sequences_need_no_pages(hip_lib):
+    """a batch padded with sequences of length 0, whose table rows hold anything"""
+    from openpvsg_amd import ops
+    ops.page_fault_check()
+    for T, longest in ((1, 40), (3, 3000)):
+        c = Cache(ops, [0, longest, 0, 17, 0], 2, 64, 16, torch.bfloat16, T)
+        c.dev_table[0], c.dev_table[2], c.dev_table[4] = -1, 1 << 30, -(1 << 31)
+        got = check(ops, c, queries((5, T, 4, 64), torch.bfloat16, T))
+        assert not bool(got[::2].any())
+        x = torch.ones(5, T, 2, 64, dtype=torch.bfloat16, device='cuda')
+        ops.kv_append(c.pages, x, x, c.dev_table, c.dev_lens)
+        k, _ = ops.kv_read(c.pages, c.dev_table, c.dev_lens, longest)
+        assert not bool(k[::2].any()) and bool((k[1, longest - T:] == 1).all())
+        ops.page_fault_check()
+
+
+@gpu
+@pytest.mark.parametrize('row,pool', ((torch.float32, torch.float32), (torch.bfloat16, torch.float8_e4m3fn)), ids=short)
+def test_both_joins_give_the_same_bits(hip_lib, row, pool):
+    """the join by the last workgroup (eager) and by a second kernel (captured): many ragged sequences, rows of one and of two tiles"""
+    from openpvsg_amd import ops
+    lens = [1 + (7919 * i) % 2500 for i in range(70)] + [6000, 0]
+    for H, G, T, D in ((2, 1, 1, 64), (1, 5, 4, 128), (1, 2, 32, 32)):
+        c = Cache(ops, lens, H, D, 32, pool, 1)
+        q = queries((len(lens), T, H * G, D), row, 2).cuda()
+        out = torch.full_like(q, 3.0)
+        eager = [ops.paged_attention(q, c.pages, c.dev_table, c.dev_lens) for _ in range(3)]
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ops.paged_attention(q, c.pages, c.dev_table, c.dev_lens, out=out)
+        for i in range(3):
+            out.fill_(3.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(bits(out), bits(eager[i]))
+        some = [0, 7, 70, 71]
+        fresh = torch.minimum(c.lens, torch.full_like(c.lens, T))
+        want, tol = reference(q.cpu()[some], [c.rows[0][b] for b in some], [c.rows[1][b] for b in some], c.lens[some], fresh[some], None, True, D ** -0.5)
+        assert bool(((out.cpu()[some].double() - want).abs() <= tol).all())
+
+
+@gpu
 def test_refusals_on_the_device(hip_lib):
     from openpvsg_amd import ops
     f = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device='cuda')  # noqa: E731
@@ -468,14 +511,17 @@ def test_refusals_on_the_device(hip_lib):
                          (f(2, 2, 8, 16, dtype=torch.int8), f(2, 2, 8, 16, dtype=torch.int8), None, None), (f(2, 2, 8, 16), f(2, 2, 8, 16), f(2, 2, 8), f(2, 2, 8)),
                          (f(2, 2, 8, 16, dtype=torch.int8), f(2, 2, 8, 16, dtype=torch.int8), f(2, 8, 2).transpose(1, 2), f(2, 2, 8)),
                          (f(2, 2, 16, 8).transpose(2, 3), f(2, 2, 16, 8).transpose(2, 3), None, None), (f(2, 2, 8, 17)[..., 1:], f(2, 2, 8, 17)[..., 1:], None, None),
-                         (f(2, 2, 1, 16).expand(2, 2, 8, 16), f(2, 2, 1, 16).expand(2, 2, 8, 16), None, None)):
+                         (f(2, 2, 1, 16).expand(2, 2, 8, 16), f(2, 2, 1, 16).expand(2, 2, 8, 16), None, None),
+                         (f(2, 1, 8, 16).expand(2, 2, 8, 16), f(2, 1, 8, 16).expand(2, 2, 8, 16), None, None),
+                         (f(1, 2, 8, 16).expand(2, 2, 8, 16), f(1, 2, 8, 16).expand(2, 2, 8, 16), None, None)):
         with pytest.raises(RuntimeError):
             ops.KVPages(k, v, ks, vs)
     p = ops.KVPages.empty(4, 2, 8, 32)
     h = ops.KVPages.empty(4, 2, 8, 32, dtype=torch.float16)
     table, lens = f(3, 2, dtype=torch.int32), f(3, dtype=torch.int32)
     x, q = f(3, 1, 2, 32), f(3, 1, 4, 32)
-    bad = [lambda: ops.kv_append(p, x, x, table.long(), lens), lambda: ops.kv_append(p, x, x, table[:2], lens), lambda: ops.kv_append(p, x, x, table, lens[:2]),
+    one = f(4, 2, 8, 32)
+    bad = [lambda: ops.kv_append(ops.KVPages(one, one), x, x, table, lens), lambda: ops.kv_append(p, x, x, table.long(), lens), lambda: ops.kv_append(p, x, x, table[:2], lens), lambda: ops.kv_append(p, x, x, table, lens[:2]),
            lambda: ops.kv_append(p, x, x.half(), table, lens), lambda: ops.kv_append(p, q, q, table, lens), lambda: ops.kv_append(p, x[0], x[0], table, lens),
            lambda: ops.kv_append(p, x.cpu(), x.cpu(), table, lens), lambda: ops.kv_append(p, x.double(), x.double(), table, lens),
            lambda: ops.kv_append(p, x, x, table.cpu(), lens), lambda: ops.kv_append(p, x, x, table, lens, new_lens=lens.long()),
