@@ -17,13 +17,16 @@ LIBNAME = 'libopenpvsg_hip.so'
 ARCH = 'gfx950'
 HIPCC = os.environ.get('HIPCC', '/opt/rocm/bin/hipcc')
 CFLAGS = ['--offload-arch=' + ARCH, '-O3', '-std=c++17', '-fPIC',
-          '-Wall', '-Wno-unused-function',
-          # no packed-f32 VALU (v_pk_add / mul / fma_f32): the vectoriser makes them from ordinary float code, and beside the
-          # MFMAs some of their forms have given wrong results on this part without an error (tests/test_mfma_hazard.py)
-          '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
-# per-file additions.  winograd3x3: what the SLP vectoriser builds (with the v_movs that feed it) beside f32 MFMAs costs issue
-# slots the scalar adds do not.
+          '-Wall', '-Wno-unused-function']
+# per-file additions.  winograd3x3: packed-f32 VALU (v_pk_add_f32 built by the SLP vectoriser, with the v_movs that feed
+# it) beside f32 MFMAs costs issue slots the scalar adds do not.
 EXTRA_CFLAGS = {'winograd3x3.hip': ['-fno-slp-vectorize']}
+# The paged cache's kernels: no packed-f32 VALU at all (the vectoriser makes it from ordinary float code; beside MFMAs some of its
+# forms have given wrong results on this part without an error, tests/test_mfma_hazard.py).  Not for the kernels above: without
+# it other products and sums of theirs contract into fmas, so every result they are known by changes in its last bits.
+NO_PACKED_F32 = ['-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops']
+for _src in ('kv_cache', 'paged_attention', 'paged_attention_f32', 'paged_attention_bf16', 'paged_attention_f16'):
+    EXTRA_CFLAGS[_src + '.hip'] = NO_PACKED_F32
 
 
 def lib_path():

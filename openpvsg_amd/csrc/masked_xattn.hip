@@ -570,7 +570,7 @@ __global__ __launch_bounds__(HW * 64, HW == 8 ? 1 : 2) void xattn_partial_bf16x3
       if (s2 > 0) { a0 = xmfma_bf16_k16(vm[0], pm[bv], a0); a1 = xmfma_bf16_k16(vm[1], pm[bv], a1); }
       const xf32x2 mref = {mrun[qc], mrun[qc]};
       if (s2 < XQT) {
-        const xf32x2 d01 = xf32x2{st[qc][0], st[qc][1]} - mref;
+        const xf32x2 d01 = xf32x2{st[qc][0], st[qc][1]} - mref;           // one v_pk_add_f32
         p01[0] = __builtin_amdgcn_exp2f(d01[0]);                          // raw v_exp_f32: arguments <= 10, and a result
         p01[1] = __builtin_amdgcn_exp2f(d01[1]);                          // below 2^-126 may flush to zero
         XPIN(p01);

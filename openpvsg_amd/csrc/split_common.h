@@ -66,7 +66,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr float F16X2_LO = 2048.f;                    // 2^11
 
 // PVSG_SPLIT_ISA (lab builds, scripts/lab/split_isa_lab.sh; profiles/r05_split_lab.txt): 0 = the form below as hipcc compiles it
-// (v_cvt_pk_f16_f32, two v_cvt_f32_f16, the residual and its scaling in scalar f32, v_cvt_pk_f16_f32);
+// (v_cvt_pk_f16_f32, two v_cvt_f32_f16, v_pk_mul_f32, v_pk_fma_f32, v_cvt_pk_f16_f32: packed f32 VALU beside the MFMAs);
 // 1 = the mixed-precision FMAs read the f16 halves directly: r = a - h by v_fma_mix_f32 (exact), l = f16(2^11 r) by
 // v_fma_mixlo_f16 / v_fma_mixhi_f16 -- five VALU instructions per pair, none packed, same bits.
 #ifndef PVSG_SPLIT_ISA
