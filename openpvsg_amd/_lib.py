@@ -226,10 +226,42 @@ except AttributeError:                    # pragma: no cover
     _cur_dev = torch.cuda.current_device
 
 
-def _stream_busy(handle):
+# A stream handle may only be asked about while the stream lives: the runtime follows a destroyed one into freed memory.  torch's own
+# streams (the default one and its pools') live as long as the process; a stream that torch was merely handed (an ExternalStream)
+# may be gone by the time the next one takes over, so behind each launch on one an event is left, which outlives it.
+_torch_owned = {0}
+_external = {}                             # device -> [handle, event behind the last launch]
+
+
+def _stream_taken(stream, dev):
+    """`stream` carries the launches of device `dev` from now on: note whose it is"""
+    if stream in _torch_owned:
+        return
+    if torch._C._cuda_getCurrentRawStream(dev) == stream and torch._C._cuda_getCurrentStream(dev)[0] & 1:   # a pool stream's id is odd
+        _torch_owned.add(stream)
+        return
+    ent = _external.get(dev)
+    if ent is None or ent[0] != stream:
+        _external[dev] = [stream, None]
+
+
+def _external_launched(stream, dev):
+    """behind a launch, where some device's launches are on a stream that is not torch's"""
+    ent = _external.get(dev)
+    if ent is None or ent[0] != stream or torch.cuda.is_current_stream_capturing():
+        return
+    if ent[1] is None:
+        ent[1] = torch.cuda.Event()
+    ent[1].record(torch.cuda.ExternalStream(stream, device=dev))
+
+
+def _stream_busy(handle, dev=None):
     """work still pending on `handle` (a stream of the CURRENT device: ops.py enters the tensor's device before it calls).
-    Only hipErrorNotReady means busy: an invalid / destroyed handle (an ExternalStream that is gone) has nothing in flight."""
+    Only hipErrorNotReady means busy.  Of a stream that is not torch's only the launches known here count."""
     global _hip
+    if handle not in _torch_owned:
+        ent = _external.get(_cur_dev() if dev is None else dev)
+        return ent is not None and ent[0] == handle and ent[1] is not None and not ent[1].query()
     if _hip is None:
         _hip = ctypes.CDLL('libamdhip64.so')          # already mapped by torch: same runtime instance
         _hip.hipStreamQuery.argtypes = [ctypes.c_void_p]
@@ -238,7 +270,7 @@ def _stream_busy(handle):
         _hip.hipGetLastError.restype = ctypes.c_int
     rc = _hip.hipStreamQuery(ctypes.c_void_p(handle))
     if rc not in (0, _HIP_ERROR_NOT_READY):
-        _hip.hipGetLastError()                        # clear the sticky error of a dead handle: it is not this launch's
+        _hip.hipGetLastError()                        # clear the sticky error: it is not this launch's
     return rc == _HIP_ERROR_NOT_READY
 
 
@@ -258,6 +290,7 @@ def _stream_changed(name, stream, ent):
             '16-bit-MFMA kernels must not share the GPU with other kernels (co-residency corruption, DESIGN.md section 3).  '
             'Keep the backend on one stream per device, or order the streams (wait_stream + synchronize) before switching; '
             'PVSG_MULTI_STREAM=allow disables this check.' % (name, stream, prev))
+    _stream_taken(stream, _cur_dev())
     ent[0], ent[1] = stream, mfma16
 
 
@@ -277,6 +310,9 @@ def note_replay(stream=None):
     if ent[0] is not None and ent[0] != stream and _stream_busy(ent[0]):
         raise ConcurrentStreamError('hipGraph replayed on HIP stream %#x while stream %#x of the same device still runs '
                                     'kernels of this backend (one stream per device)' % (stream, ent[0]))
+    _stream_taken(stream, dev)
+    if _external:
+        _external_launched(stream, dev)
     ent[0], ent[1] = stream, True
 
 
@@ -296,6 +332,8 @@ def call(name, *args):
         elif not ent[1] and name in _MFMA16_NAMES:
             ent[1] = True
     rc = getattr(lib, name)(*args)
+    if _external and _CHECK_STREAMS:
+        _external_launched(args[-1] or 0, _cur_dev())
     if rc != 0:
         msg = lib.pvsg_last_error()
         raise RuntimeError('%s failed (code %d): %s' % (name, rc, msg.decode() if msg else '?'))
