@@ -148,6 +148,13 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppend a) {
   // workgroups, each behind another L2, cost as much as the codes (measured at 16 x 4096 rows into int8: 93 -> 86 us)
   const unsigned r = (blockIdx.x << (8 - a.lanes_shift)) + (threadIdx.x >> a.lanes_shift), run = r >> a.run_shift;
   const unsigned t = ((run / a.p.heads) << a.run_shift) + (r & ((1u << a.run_shift) - 1)), h = run % a.p.heads;
+  // the rows are asked for before the lengths and the page id are there: a row that turns out not to be real is not written
+  unsigned kr[RB * 2] = {}, vr[RB * 2] = {};
+  if ((int)t < a.T) {
+    const long long src = b * a.seq_stride + (long long)t * a.token_stride + (long long)h * a.head_stride;
+    kv_load_run<RT, kv_run(RT, CT)>(kr, a.k + src, sub, lanes, a.p.dim);
+    kv_load_run<RT, kv_run(RT, CT)>(vr, a.v + src, sub, lanes, a.p.dim);
+  }
   const KvSpan span = kv_span(a.lens, a.new_lens, b, a.T, a.width << a.page_shift);
   bool live = (int)t < span.fresh;
   const int pos = live ? span.len - span.fresh + (int)t : 0;
@@ -159,12 +166,6 @@ __global__ __launch_bounds__(256) void kv_append_kernel(const KvAppend a) {
       page = 0;
       if (sub == 0) kv_fault(a.p.faults, 1);
     }
-  }
-  unsigned kr[RB * 2] = {}, vr[RB * 2] = {};
-  if (live) {
-    const long long src = b * a.seq_stride + (long long)t * a.token_stride + (long long)h * a.head_stride;
-    kv_load_run<RT, kv_run(RT, CT)>(kr, a.k + src, sub, lanes, a.p.dim);
-    kv_load_run<RT, kv_run(RT, CT)>(vr, a.v + src, sub, lanes, a.p.dim);
   }
   const int slot = pos & (a.p.page_size - 1);
   const long long dst = ((long long)page * a.p.page_stride + (long long)h * a.p.head_stride + (long long)slot * a.p.slot_stride) * CB;

@@ -62,7 +62,7 @@ __device__ __forceinline__ const __attribute__((address_space(4))) int* pa_const
 }
 
 // workgroups of a CU that the kernel's registers leave room for
-constexpr int pa_per_cu(int dim, int tiles) { return dim <= 32 ? 4 : dim <= 64 ? (tiles == 1 ? 3 : 2) : dim <= 128 ? 2 : 1; }
+constexpr int pa_per_cu(int dim, int tiles) { return dim <= 64 ? (tiles == 1 ? 3 : 2) : dim <= 128 ? 2 : 1; }
 
 // four packed 16-bit words (the 8 elements of one lane of a matrix product's operand)
 template <int MT>
@@ -111,6 +111,17 @@ __device__ __forceinline__ float pa_max4(float x) {
 __device__ __forceinline__ float pa_sum4(float x) {
   x += __shfl_xor(x, 16);
   return x + __shfl_xor(x, 32);
+}
+
+// sum over the lanes up to this one: inside the 16-lane rows by shifts, then the last lane of a row (of two rows) to the next
+__device__ __forceinline__ unsigned pa_scan(unsigned x) {
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true);
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true);
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true);
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true);
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);
+  x += (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);
+  return x;
 }
 
 template <int RT>
@@ -224,6 +235,7 @@ __device__ void pa_rows_alone(PagedAttnArgs& a, int b, int h, int lo, int hi, in
       if (page >= 0) {
         const long long at = (long long)page * a.p.page_stride + (long long)h * a.p.head_stride + (long long)slot * a.p.slot_stride;
         z = 0.f;
+#pragma unroll 1
         for (int d = 0; d < D; d += 8) {
           unsigned kw[8], qw[8];
           kv_load<kv_bytes(CT) == 4 ? 16 : kv_bytes(CT) * 8>(kw, static_cast<const unsigned char*>(a.p.k) + (at + d) * kv_bytes(CT));
@@ -241,6 +253,7 @@ __device__ void pa_rows_alone(PagedAttnArgs& a, int b, int h, int lo, int hi, in
       z_of[tid] = z;
       __syncthreads();
       float up = top;
+#pragma unroll 4
       for (int i = 0; i < 256; ++i) up = fmaxf(up, z_of[i]);
       const float ref = up == -INFINITY ? 0.f : up;
       const float shrink = __builtin_amdgcn_exp2f(top - ref);
@@ -249,6 +262,7 @@ __device__ void pa_rows_alone(PagedAttnArgs& a, int b, int h, int lo, int hi, in
       __syncthreads();
       // (before anything was seen o and sum are 0, and shrink is 0 or 1)
       o *= shrink, sum *= shrink;
+#pragma unroll 1
       for (int i = 0; i < min(256, lim - p0); ++i) {
         if (page_of[i] < 0) continue;
         const int si = (p0 + i) & (a.p.page_size - 1);
@@ -333,12 +347,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
     for (int k = 0; k < 4; ++k) mine += b0 + k < b1 ? PA_PART + tiles_of(lens[k], capacity) : 0;
     for (int i = b0 + 4; i < b1; ++i) mine += PA_PART + tiles_of(a.lens[i], capacity);
     mine *= each;
-    unsigned upto = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const unsigned x = __shfl_up(upto, o);
-      if (lane >= o) upto += x;
-    }
+    const unsigned upto = pa_scan(mine);
     const unsigned total = __builtin_amdgcn_readlane(upto, 63);
     const unsigned used = min((unsigned)a.workgroups, (total + PA_PART + PA_GRAIN - 1) / (PA_PART + PA_GRAIN));
     share = total / used, more = total - share * used;
@@ -399,6 +408,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
       if (!a.arrived && tile0 == 0 && tid == 0) a.part_of[3 * blockIdx.x] = b, a.part_of[3 * blockIdx.x + 1] = hr, a.part_of[3 * blockIdx.x + 2] = last_wg;
     }
     const int h = hr / a.row_groups, row0 = hr % a.row_groups * (16 * NT);
+    const int fresh = a.new_lens ? pa_const(a.new_lens)[b] : a.T;
 
     // what depends on the length alone is asked for first: the page ids of the first keys, two a thread at most
     const int there = min(max(len, 0), capacity), key1 = (int)min((long long)tile1 * TILE, (long long)there);
@@ -438,7 +448,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
       }
     }
 
-    const KvSpan span = kv_span_of(len, a.new_lens ? pa_const(a.new_lens)[b] : a.T, a.T, capacity);
+    const KvSpan span = kv_span_of(len, fresh, a.T, capacity);
     const int past = span.len - span.fresh;
     if (len > capacity && tid == 0) kv_fault(a.p.faults, 4);
     // what the first and the last real row of this group see, and each of this lane's

@@ -1617,7 +1617,7 @@ class KVPages:
     (float8_e4m3fn, int8) with a float32 scale per row, k_scale / v_scale (num_pages, heads, page_size), contiguous.
     Slots hold x, 8-bit ones x / scale.  The pool is written in place by `kv_append`; its tensors stay the caller's."""
 
-    __slots__ = ('k', 'v', 'k_scale', 'v_scale', 'dtype', 'device', 'num_pages', 'heads', 'page_size', 'head_dim', '_struct')
+    __slots__ = ('k', 'v', 'k_scale', 'v_scale', 'dtype', 'device', 'index', 'num_pages', 'heads', 'page_size', 'head_dim', '_struct')
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         for n, t in (('k', k), ('v', v)):
@@ -1652,7 +1652,8 @@ class KVPages:
                 if _chk(t, 'KVPages: ' + n).data_ptr() != t.data_ptr() or tuple(t.shape) != (P, H, S) or t.device != k.device or t.data_ptr() & 15:
                     raise RuntimeError('KVPages: %s must be contiguous (num_pages, heads, page_size) on the pool\'s device' % n)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.dtype, self.device, self.num_pages, self.heads, self.page_size, self.head_dim = k.dtype, k.device, P, H, S, D
+        self.dtype, self.device, self.index = k.dtype, k.device, k.get_device()
+        self.num_pages, self.heads, self.page_size, self.head_dim = P, H, S, D
         self._struct = _lib.KvPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if scaled else None,
                                     v_scale.data_ptr() if scaled else None, sp, sh, ss, H * S, S, P, H, S, D,
                                     _KV_TYPES[k.dtype], _page_fault_word(k.device).data_ptr())
@@ -1668,22 +1669,21 @@ class KVPages:
 
 def _kv_ints(t, name, pages, B):
     """(B,) int32 on the pool's device, dense"""
-    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != pages.device or t.shape != (B,):
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.get_device() != pages.index or t.shape != (B,):
         raise RuntimeError('%s must be an int32 tensor of shape (%d,) on %s' % (name, B, pages.device))
     return t if B < 2 or t.stride(0) == 1 else t.contiguous()
 
 
 def _kv_table(t, pages, B):
     """(B, W) int32 page table with dense rows -> tensor, row stride, W"""
-    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != pages.device or t.dim() != 2 or B not in (None, t.shape[0]):
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.get_device() != pages.index or t.dim() != 2 or B not in (None, t.shape[0]):
         raise RuntimeError('table must be an int32 tensor of shape (%s, pages) on %s' % ('?' if B is None else B, pages.device))
     W = t.shape[1]
     if W < 1 or W * pages.page_size > 1 << 30:
         raise RuntimeError('table: %d pages of %d positions (one page at least, 2^30 positions at most)' % (W, pages.page_size))
     row, one = t.stride()
     if W > 1 and one != 1:
-        t = t.contiguous()
-        row = W
+        t, row = t.contiguous(), W
     return t, row, W
 
 
@@ -1697,7 +1697,7 @@ def _kv_rows(t, name, pages, heads):
     """(B, T, heads, head_dim) rows of an activation type, any strides; copied where a row is not dense or not 16-byte aligned"""
     if not isinstance(t, torch.Tensor) or t.dim() != 4:
         raise RuntimeError('%s must be a (sequences, tokens, heads, head_dim) tensor' % name)
-    if t.device != pages.device:
+    if t.get_device() != pages.index:
         if not t.is_cuda:
             raise RuntimeError('%s must live on a HIP device (got %s); the MI355X backend has no CPU path' % (name, t.device))
         raise RuntimeError('%s is on %s, the pool on %s' % (name, t.device, pages.device))
@@ -1724,8 +1724,7 @@ def kv_append(pages, k, v, table, lens, new_lens=None):
     n = min(T, lens[b], new_lens[b]) are written, at positions lens[b] - n ..; new_lens (B,) int32 defaults to T everywhere.
     8-bit pools: scale = max(max|row| * (1/448 or 1/127), 2^-126), code = round(row / scale), ties to even; a row with a NaN or infinity reads
     back as NaN.  Pages that are appended to belong to one sequence.  Page ids out of the pool: skipped, see page_fault_check."""
-    k = _kv_rows(k, 'k', pages, pages.heads)
-    v = _kv_rows(v, 'v', pages, pages.heads)
+    k, v = _kv_rows(k, 'k', pages, pages.heads), _kv_rows(v, 'v', pages, pages.heads)
     if pages.k.data_ptr() == pages.v.data_ptr():
         raise RuntimeError('kv_append: the pool\'s k and v are the same memory')
     if k.shape != v.shape or k.dtype != v.dtype:
@@ -1775,7 +1774,7 @@ def _paged_attention_counters(device, stream):
     """Zeroed words by which the workgroups of a launch find out who joins a split row: one set for each stream, whose launches
     follow each other and leave them zero.  None while a graph is captured: its replays may run beside anything, so a second
     launch joins there."""
-    if torch.cuda.is_current_stream_capturing():
+    if torch._C._cuda_isCurrentStreamCapturing():
         return None
     t = _attention_counters.get((device, stream))
     if t is None:
@@ -1814,7 +1813,7 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
             mask = mask.contiguous()
         ms, mw = mask.stride(0), mask.shape[1]
     if out is None:
-        out = q.new_empty((B, T, HQ, D))
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, T, HQ, D))
     elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or \
             out.data_ptr() & 15 or out.requires_grad:
         raise RuntimeError('paged_attention: out must be a contiguous, 16-byte aligned %s tensor of shape %s on %s' % (q.dtype, tuple(q.shape), q.device))
@@ -1831,5 +1830,5 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
         _lib.call('pvsg_paged_attention', pages._struct, q.data_ptr(), sb, st, sh, out.data_ptr(), row, table.data_ptr(), table_row, width,
                   lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, mask.data_ptr() if mask is not None else None,
                   ms, mw, B, T, HQ, D ** -0.5 if scale is None else float(scale), 1 if causal else 0, longest,
-                  work.data_ptr() if work is not None else None, _paged_attention_counters(q.device.index, stream) if nbytes else None, stream)
+                  work.data_ptr() if work is not None else None, _paged_attention_counters(pages.index, stream) if nbytes else None, stream)
     return out

@@ -34,7 +34,7 @@ def test_a_busy_external_stream_is_seen_and_a_destroyed_one_is_idle(hip_lib):
     torch.cuda.synchronize()
     hip = ctypes.CDLL('libamdhip64.so')
     stream = ctypes.c_void_p()
-    assert hip.hipStreamCreate(ctypes.byref(stream)) == 0
+    assert hip.hipStreamCreateWithFlags(ctypes.byref(stream), 1) == 0          # not a blocking one: the default stream's query waits for those
     with torch.cuda.stream(torch.cuda.ExternalStream(stream.value)):
         for _ in range(20):
             ops.gemm_bf16x3(a, wp, 1024, out=out)
