@@ -687,8 +687,8 @@ int pvsg_kv_read(const pvsg_kv_pages* pages, void* k_out, void* v_out, int out_t
  * once; a row that sees nothing, or past n_b, is zero.  What a row does not see does not reach it, NaN and infinities included.
  * max_len: the longest cache to plan for (0: what the table holds); longer ones are computed all the same.
  * workspace: pvsg_paged_attention_workspace_bytes of the same arguments (0: none), 16-byte aligned, no initialisation.
- * counters: NULL, or PVSG_PAGED_ATTENTION_COUNTERS words that were zero before the first call that was given them and that no two calls
- * in flight share; every call leaves them zero.  With them the parts of a split row are joined in the same launch, without in a second one. */
+ * counters: needed with a workspace: PVSG_PAGED_ATTENTION_COUNTERS words that were zero before the first call that was given them and that no two
+ * calls in flight share; every call leaves them zero. */
 #define PVSG_PAGED_ATTENTION_COUNTERS 1024
 long long pvsg_paged_attention_workspace_bytes(const pvsg_kv_pages* pages, int B, int T, int q_heads, int row_type, int table_width,
                                                long long max_len);

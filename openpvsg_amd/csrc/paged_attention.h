@@ -11,8 +11,8 @@
 //
 // Sequences differ in length, and only the device knows by how much.  So the tiles of all of them are one list, and as many
 // workgroups as the card holds each take an equal stretch of it: each finds its stretch by a scan over the lengths.  A (sequence, key
-// head, row group) that lies in several stretches leaves (m, l, O) of each, and a second kernel joins them.  Where no cache is
-// longer than a few tiles there is nothing to even out, and each has a workgroup of its own and no join.
+// head, row group) that lies in several stretches leaves (m, l, O) of each, and whoever comes last joins them, in the stretches' order.  Where
+// no cache is longer than a few tiles there is nothing to even out, and each has a workgroup of its own and no join.
 //
 // Rounding: 16-bit rows multiply in their own type, exact products in f32 sums; 8-bit codes convert to it exactly and their
 // scales multiply S and P in f32.  P goes to the matrix cores as a 16-bit high part plus a 16-bit rest (one part alone adds an error as
@@ -42,8 +42,7 @@ struct PagedAttn {
   int width, padding_width, page_shift;
   int B, T, q_heads, group, rows, row_groups, causal;
   int workgroups;                        // how many share the tiles; 0: one for each (sequence, key head, row group)
-  int* part_of;                          // of each: the sequence, the key head and row group, and the last workgroup that it splits with
-  unsigned* arrived;                     // zeros, one for each: the last workgroup of a row joins its parts; null: a second kernel does
+  unsigned* arrived;                     // zeros, one for each: how many parts of a row are there
 };
 
 constexpr int PA_WAVES = 4;
@@ -137,16 +136,10 @@ __device__ __forceinline__ void pa_store_row4(unsigned char* out, long long at, 
   }
 }
 
-// A part's values between workgroups.  FRESH: written in this launch, so they are read past the caches that other workgroups' stores do
-// not reach.
-template <bool FRESH>
-__device__ __forceinline__ float2 pa_part2(const float* p) {
-  if constexpr (FRESH) {
-    const unsigned long long u = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    return make_float2(__builtin_bit_cast(float, (unsigned)u), __builtin_bit_cast(float, (unsigned)(u >> 32)));
-  } else {
-    return *reinterpret_cast<const float2*>(p);
-  }
+// A part's values go between workgroups of one launch: stored through and read past the caches that other workgroups do not share.
+__device__ __forceinline__ float2 pa_get2(const float* p) {
+  const unsigned long long u = __hip_atomic_load(reinterpret_cast<const unsigned long long*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return make_float2(__builtin_bit_cast(float, (unsigned)u), __builtin_bit_cast(float, (unsigned)(u >> 32)));
 }
 __device__ __forceinline__ void pa_put2(float* p, float x, float y) {
   const unsigned long long u = __builtin_bit_cast(unsigned, x) | (unsigned long long)__builtin_bit_cast(unsigned, y) << 32;
@@ -155,8 +148,8 @@ __device__ __forceinline__ void pa_put2(float* p, float x, float y) {
 // The parts that the stretches of workgroups first .. first + n - 1 left of the `tile_rows` rows at row0 of key head h: joined and written.
 // dim / 4 threads across a row; of the groups of so many threads, `share` take one row's parts between them, so that few rows of
 // many parts are read at once as well.  The parts come in the stretches' order, whoever joins them.
-template <int RT, bool FRESH, class A>
-__device__ void pa_join(A& a, int b, int h, int row0, int tile_rows, int first, int n, int fresh, float (*s_o)[4], float* s_m, float* s_l) {
+template <int RT>
+__device__ void pa_join(PagedAttnArgs& a, int b, int h, int row0, int tile_rows, int first, int n, int fresh, float (*s_o)[4], float* s_m, float* s_l) {
   const int rows = min(tile_rows, a.rows - row0);
   const int D = a.p.dim, d4 = D / 4, groups = 256 / d4, x = threadIdx.x % d4, y = threadIdx.x / d4;
   const int share = max(1, min(groups / rows, n / 2)), at_once = groups / share;
@@ -169,8 +162,8 @@ __device__ void pa_join(A& a, int b, int h, int row0, int tile_rows, int first, 
 #pragma unroll 4
       for (int k = k0; k < n; k += share) {
         const long long slot = (long long)(2 * (first + k) + (k == 0 ? 1 : 0)) * tile_rows + r;
-        const float2 p = pa_part2<FRESH>(a.part_ml + 2 * slot);
-        const float2 v = pa_part2<FRESH>(a.part_o + slot * D + 4 * x), u = pa_part2<FRESH>(a.part_o + slot * D + 4 * x + 2);
+        const float2 p = pa_get2(a.part_ml + 2 * slot);
+        const float2 v = pa_get2(a.part_o + slot * D + 4 * x), u = pa_get2(a.part_o + slot * D + 4 * x + 2);
         const float up = fmaxf(top, p.x), ref = up == -INFINITY ? 0.f : up;
         const float keep = __builtin_amdgcn_exp2f(top - ref), w = __builtin_amdgcn_exp2f(p.x - ref);
         sum = sum * keep + w * p.y;
@@ -352,7 +345,6 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
     const unsigned used = min((unsigned)a.workgroups, (total + PA_PART + PA_GRAIN - 1) / (PA_PART + PA_GRAIN));
     share = total / used, more = total - share * used;
     first = blockIdx.x * share + min(blockIdx.x, more);
-    if (!a.arrived && threadIdx.x == 0) a.part_of[3 * blockIdx.x] = -1;
     if (blockIdx.x >= used) return;
     left = share + (blockIdx.x < more ? 1 : 0);
     const int whose = __builtin_ctzll(__ballot(first < upto));      // the lane whose sequences the stretch begins in
@@ -405,7 +397,6 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
       const int slot = 2 * blockIdx.x + (tile0 == 0 ? 1 : 0);
       part_o = a.part_o + (long long)slot * (16 * NT) * D;
       part_ml = a.part_ml + (long long)slot * (16 * NT) * 2;
-      if (!a.arrived && tile0 == 0 && tid == 0) a.part_of[3 * blockIdx.x] = b, a.part_of[3 * blockIdx.x + 1] = hr, a.part_of[3 * blockIdx.x + 2] = last_wg;
     }
     const int h = hr / a.row_groups, row0 = hr % a.row_groups * (16 * NT);
     const int fresh = a.new_lens ? pa_const(a.new_lens)[b] : a.T;
@@ -759,7 +750,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
       __syncthreads();
       pa_rows_alone<RT, CT>(a, b, h, tile0 * TILE, most, row0, min(row0 + 16 * NT, a.rows), span, part_o, part_ml, &s_o[0][0][0]);
     }
-    if (a.arrived && part_o) {
+    if (part_o) {
       // The last of a row's workgroups joins its parts.  Parts are stored through the caches that do not reach other workgroups, and
       // every store is complete before this one counts; a release at device scope would write back everything those caches hold
       // (measured: microseconds).  The counter is zero again for the next launch.
@@ -776,7 +767,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
       __syncthreads();
       if (last) {
         float* buf = &s_o[0][0][0];
-        pa_join<RT, true>(a, b, h, row0, 16 * NT, first_wg, last_wg - first_wg + 1, span.fresh, reinterpret_cast<float(*)[4]>(buf), buf + 1024, buf + 1280);
+        pa_join<RT>(a, b, h, row0, 16 * NT, first_wg, last_wg - first_wg + 1, span.fresh, reinterpret_cast<float(*)[4]>(buf), buf + 1024, buf + 1280);
         __syncthreads();
       }
     }

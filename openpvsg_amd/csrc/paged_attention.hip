@@ -1,20 +1,7 @@
-// Entry points of the paged attention (paged_attention.h has the kernel and its reasons) and the join of its splits.
+// Entry points of the paged attention (paged_attention.h has the kernel and its reasons).
 #include "paged_attention.h"
 
 namespace pvsg {
-
-// The join as a kernel of its own: workgroup i looks at the part that workgroup i of the first kernel left of a row that ends in a later
-// stretch.
-template <int RT>
-__global__ __launch_bounds__(256) void paged_attention_join_kernel(const PagedAttn a, int tile_rows) {
-  __shared__ __align__(16) float s_o[256][4];
-  __shared__ float s_m[256], s_l[256];
-  const int first = blockIdx.x, b = a.part_of[3 * first];
-  if (b < 0) return;
-  const int hr = a.part_of[3 * first + 1], n = a.part_of[3 * first + 2] - first + 1;
-  const KvSpan span = kv_span(a.lens, a.new_lens, b, a.T, a.width << a.page_shift);
-  pa_join<RT, false>(a, b, hr / a.row_groups, hr % a.row_groups * tile_rows, tile_rows, first, n, span.fresh, s_o, s_m, s_l);
-}
 
 // Caches of up to so many tiles are not split: each has a workgroup of its own.  Measured over 4 .. 800 (sequence, key head)s of bf16
 // heads of 128: at 700 positions (6 tiles) 11.0 - 37.8 us so and 13.5 - 42.8 us split and joined, at 1000 (8) 13.5 - 50 and 13.7 -
@@ -28,7 +15,7 @@ static int pa_tiles(int rows, int dim, int row_type) { return rows > 16 && dim <
 struct PaPlan {
   int tiles, row_groups, workgroups;
   long long units;
-  size_t part_o, part_ml, part_of;       // floats, floats, ints of the workspace
+  size_t part_o, part_ml;                // floats of the workspace
 };
 static PaPlan pa_plan(const pvsg_kv_pages& p, int B, int T, int q_heads, int row_type, int table_width, long long max_len) {
   PaPlan s{};
@@ -44,7 +31,7 @@ static PaPlan pa_plan(const pvsg_kv_pages& p, int B, int T, int q_heads, int row
   const long long room = 256 * pa_per_cu(p.dim, s.tiles), work = (s.units * (tiles + PA_PART) + PA_PART + PA_GRAIN - 1) / (PA_PART + PA_GRAIN);
   s.workgroups = (int)(work < room ? work : room);
   const size_t rows_of = (size_t)2 * s.workgroups * 16 * s.tiles;
-  s.part_o = rows_of * p.dim, s.part_ml = rows_of * 2, s.part_of = (size_t)3 * s.workgroups;
+  s.part_o = rows_of * p.dim, s.part_ml = rows_of * 2;
   return s;
 }
 
@@ -55,7 +42,7 @@ extern "C" long long pvsg_paged_attention_workspace_bytes(const pvsg_kv_pages* p
   using namespace pvsg;
   if (!pages || pages->heads <= 0 || pages->dim <= 0 || B <= 0 || T <= 0 || q_heads < pages->heads || table_width <= 0) return 0;
   const PaPlan s = pa_plan(*pages, B, T, q_heads, row_type, table_width, max_len);
-  return (long long)(s.part_o + s.part_ml + s.part_of) * 4;
+  return (long long)(s.part_o + s.part_ml) * 4;
 }
 
 extern "C" int pvsg_paged_attention(const pvsg_kv_pages* pages, const void* q, long long q_seq_stride, long long q_token_stride,
@@ -74,8 +61,9 @@ extern "C" int pvsg_paged_attention(const pvsg_kv_pages* pages, const void* q, l
   PVSG_REQUIRE(!padding || (padding_width >= 0 && padding_stride >= 0), "pvsg_paged_attention: bad padding mask");
   if (B == 0 || T == 0) return PVSG_OK;
   const PaPlan s = pa_plan(*pages, B, T, q_heads, row_type, table_width, max_len);
-  PVSG_REQUIRE(s.workgroups == 0 || (workspace && ((uintptr_t)workspace & 15) == 0), "pvsg_paged_attention: workspace %p, %lld bytes are needed", workspace,
-               (long long)(s.part_o + s.part_ml + s.part_of) * 4);
+  PVSG_REQUIRE(s.workgroups == 0 || (workspace && counters && (((uintptr_t)workspace & 15) | ((uintptr_t)counters & 3)) == 0),
+               "pvsg_paged_attention: workspace %p and counters %p, %lld bytes are needed", workspace, static_cast<void*>(counters),
+               (long long)(s.part_o + s.part_ml) * 4);
   PVSG_REQUIRE(s.units < (1ll << 31), "pvsg_paged_attention: %lld parts are too many for one launch", s.units);
   PagedAttn a{};
   a.p = *pages;
@@ -91,18 +79,10 @@ extern "C" int pvsg_paged_attention(const pvsg_kv_pages* pages, const void* q, l
   if (s.workgroups) {
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + s.part_o;
-    a.part_of = reinterpret_cast<int*>(a.part_ml + s.part_ml);
     a.arrived = counters;
   }
   const hipStream_t st = static_cast<hipStream_t>(stream);
   (row_type == KV_F32 ? pa_run_f32 : row_type == KV_BF16 ? pa_run_bf16 : pa_run_f16)(a, s.tiles, (unsigned)(s.workgroups ? s.workgroups : s.units), st);
   PVSG_LAUNCH_CHECK("pvsg_paged_attention");
-  if (s.workgroups > 1 && !counters) {
-    const dim3 grid((unsigned)(s.workgroups - 1));
-    if (row_type == KV_F32) hipLaunchKernelGGL((paged_attention_join_kernel<KV_F32>), grid, dim3(256), 0, st, a, 16 * s.tiles);
-    else if (row_type == KV_BF16) hipLaunchKernelGGL((paged_attention_join_kernel<KV_BF16>), grid, dim3(256), 0, st, a, 16 * s.tiles);
-    else hipLaunchKernelGGL((paged_attention_join_kernel<KV_F16>), grid, dim3(256), 0, st, a, 16 * s.tiles);
-    PVSG_LAUNCH_CHECK("pvsg_paged_attention");
-  }
   return PVSG_OK;
 }

@@ -1772,14 +1772,14 @@ _attention_counters = {}
 
 def _paged_attention_counters(device, stream):
     """Zeroed words by which the workgroups of a launch find out who joins a split row: one set for each stream, whose launches
-    follow each other and leave them zero.  None while a graph is captured: its replays may run beside anything, so a second
-    launch joins there."""
+    follow each other and leave them zero.  A launch that is captured gets its own, cleared in the graph: replays may run beside
+    anything."""
     if torch._C._cuda_isCurrentStreamCapturing():
-        return None
+        return torch.zeros(1024, dtype=torch.int32, device=torch.device('cuda', device))
     t = _attention_counters.get((device, stream))
     if t is None:
         t = _attention_counters[device, stream] = torch.zeros(1024, dtype=torch.int32).to(torch.device('cuda', device))
-    return t.data_ptr()
+    return t
 
 
 def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None, causal=True, scale=None, max_len=None, out=None):
@@ -1827,8 +1827,9 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
     sb, st, sh, _ = q.stride()
     with _on(pages.device):
         stream = _stream_ptr()
+        counters = _paged_attention_counters(pages.index, stream) if nbytes else None
         _lib.call('pvsg_paged_attention', pages._struct, q.data_ptr(), sb, st, sh, out.data_ptr(), row, table.data_ptr(), table_row, width,
                   lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, mask.data_ptr() if mask is not None else None,
                   ms, mw, B, T, HQ, D ** -0.5 if scale is None else float(scale), 1 if causal else 0, longest,
-                  work.data_ptr() if work is not None else None, _paged_attention_counters(pages.index, stream) if nbytes else None, stream)
+                  work.data_ptr() if work is not None else None, counters.data_ptr() if nbytes else None, stream)
     return out
