@@ -47,7 +47,6 @@ struct PagedAttn {
 
 constexpr int PA_WAVES = 4;
 constexpr int PA_CHUNK = 4096;           // keys whose pages are looked up at a time
-constexpr int PA_PART = 3;                // what a part costs beside its tiles, in tiles
 constexpr int PA_GRAIN = 1;               // tiles that a workgroup takes at least
 constexpr int PA_MAX_T = 32;
 
@@ -60,8 +59,21 @@ __device__ __forceinline__ const __attribute__((address_space(4))) int* pa_const
   return (const __attribute__((address_space(4))) int*)p;
 }
 
+// whether rows of one type over a pool of another are multiplied in 16 bits
+constexpr bool pa_16bit(int row, int pool) { return row != KV_F32 || pool == KV_BF16 || kv_scaled(pool); }
+// the size class of a head
+constexpr int pa_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
+// 16-key blocks of a wave's tile.  f32 products take one key at a time, so that a block of theirs is work enough.  Of heads of up to 64
+// in 16 bits there is room for four beside the next tile's, and where the caches are long (`split`: the tiles are shared out) they
+// save waits for memory: 64 x 8192 x 8 heads of 64 int8 123 -> 112 us, 20 ragged ones of up to 3000 18.0 -> 15.6.  Short ones go two blocks at a time,
+// three workgroups to a CU: 100 of up to 900 positions 19.3 us, and 22.3 with four.
+constexpr int pa_blocks(int row, int pool, int dim, int tiles, bool split) {
+  return pa_16bit(row, pool) ? (split && tiles == 1 && row != KV_F32 && dim <= 64 ? 4 : 2) : dim <= 32 ? 2 : 1;
+}
+// what a part costs beside its tiles, in tiles (swept 1 .. 5)
+constexpr int pa_part_cost(int blocks) { return blocks == 4 ? 1 : 3; }
 // workgroups of a CU that the kernel's registers leave room for
-constexpr int pa_per_cu(int dim, int tiles) { return dim <= 64 ? (tiles == 1 ? 3 : 2) : dim <= 128 ? 2 : 1; }
+constexpr int pa_per_cu(int dim, int tiles, int blocks) { return dim <= 64 ? (tiles == 1 && blocks < 4 ? 3 : 2) : dim <= 128 ? 2 : 1; }
 
 // four packed 16-bit words (the 8 elements of one lane of a matrix product's operand)
 template <int MT>
@@ -295,14 +307,13 @@ __device__ __forceinline__ void pa_parts(float a, float b, unsigned (&w)[PARTS])
   }
 }
 
-template <int RT, int CT, int DP, int NT, bool PADDED>
-__global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attention_kernel(const PagedAttn) {
-  constexpr bool M16 = RT != KV_F32 || CT == KV_BF16 || kv_scaled(CT);
+template <int RT, int CT, int DP, int NT, int KT, bool PADDED>
+__global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT, KT)) void paged_attention_kernel(const PagedAttn) {
+  constexpr bool M16 = pa_16bit(RT, CT);
   constexpr int QK = RT == KV_F16 ? KV_F16 : KV_BF16, PV = CT == KV_F16 ? KV_F16 : KV_BF16;      // operand types of the 16-bit products
   constexpr int QL = RT == KV_F32 ? 3 : 1, PL = RT == KV_F32 ? 3 : 2;
   constexpr int CB = kv_bytes(CT), RB = kv_bytes(RT);
-  constexpr int KT = M16 || DP <= 32 ? 2 : 1;                       // 16-key blocks of a tile
-  constexpr int KEYS = 16 * KT;
+  constexpr int KEYS = 16 * KT, PA_PART = pa_part_cost(KT);           // a wave's tile is KT blocks of 16 keys
   // keys: chunk i of a lane in 16-lane group g is columns i*4*KC + KC*g ...; values: column c*16*VC + VC*m + e for lane m
   constexpr int KC = 16 / CB < DP / 4 ? 16 / CB : DP / 4, NK = DP / (4 * KC), KW = KC * CB / 4;
   constexpr int VE = DP / 16, VC = 16 / CB < VE ? 16 / CB : VE, NV = VE / VC, VB = VC * CB, VW = (VB + 3) / 4;
@@ -620,53 +631,56 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
 
         // ---- O^T += V^T P^T
         if constexpr (M16) {
-          unsigned pf[NT][PL][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int k0 = 0; k0 < KT * 4; k0 += 8) {                    // eight of this lane's keys at a time
+            unsigned pf[NT][PL][4];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              unsigned part[PL];
-              pa_parts<PL, PV>(pr[nt][2 * x], pr[nt][2 * x + 1], part);
-#pragma unroll
-              for (int l = 0; l < PL; ++l) pf[nt][l][x] = part[l];
-            }
-#pragma unroll
-          for (int c = 0; c < NV; ++c) {
-#pragma unroll
-            for (int q4 = 0; q4 < (VC + 3) / 4; ++q4) {
-              // four columns (a pair of words of 16-bit elements, a word of codes) of eight keys -> one operand per column
-              unsigned vf[4][4];
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int x = 0; x < 4; ++x) {
-                if constexpr (CB == 2) {
+                unsigned part[PL];
+                pa_parts<PL, PV>(pr[nt][k0 + 2 * x], pr[nt][k0 + 2 * x + 1], part);
 #pragma unroll
-                  for (int y = 0; y < 2; ++y) {
-                    if (4 * q4 + 2 * y < VC) {
-                      const unsigned wa = vw[2 * x][c * VW + 2 * q4 + y], wb = vw[2 * x + 1][c * VW + 2 * q4 + y];
-                      vf[2 * y][x] = __builtin_amdgcn_perm(wb, wa, 0x05040100u);
-                      vf[2 * y + 1][x] = __builtin_amdgcn_perm(wb, wa, 0x07060302u);
-                    }
-                  }
-                } else {
-                  const unsigned wa = vw[2 * x][c * VW + q4], wb = vw[2 * x + 1][c * VW + q4];
-                  const unsigned t0 = __builtin_amdgcn_perm(wb, wa, 0x05010400u), t1 = __builtin_amdgcn_perm(wb, wa, 0x07030602u);
-                  vf[0][x] = pa_widen<PV, CT>(t0, false);
-                  vf[1][x] = pa_widen<PV, CT>(t0, true);
-                  if (VC > 2) {
-                    vf[2][x] = pa_widen<PV, CT>(t1, false);
-                    vf[3][x] = pa_widen<PV, CT>(t1, true);
-                  }
-                }
+                for (int l = 0; l < PL; ++l) pf[nt][l][x] = part[l];
               }
 #pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                if (4 * q4 + y < VC) {
-                  const int e = c * VC + 4 * q4 + y;
+            for (int c = 0; c < NV; ++c) {
 #pragma unroll
-                  for (int nt = 0; nt < NT; ++nt)
+              for (int q4 = 0; q4 < (VC + 3) / 4; ++q4) {
+                // four columns (a pair of words of 16-bit elements, a word of codes) of the keys -> one operand per column
+                unsigned vf[4][4];
 #pragma unroll
-                    for (int l = 0; l < PL; ++l) acc[nt][e] = pa_mfma16<PV>(vf[y], pf[nt][l], acc[nt][e]);
+                for (int x = 0; x < 4; ++x) {
+                  if constexpr (CB == 2) {
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                      if (4 * q4 + 2 * y < VC) {
+                        const unsigned wa = vw[k0 + 2 * x][c * VW + 2 * q4 + y], wb = vw[k0 + 2 * x + 1][c * VW + 2 * q4 + y];
+                        vf[2 * y][x] = __builtin_amdgcn_perm(wb, wa, 0x05040100u);
+                        vf[2 * y + 1][x] = __builtin_amdgcn_perm(wb, wa, 0x07060302u);
+                      }
+                    }
+                  } else {
+                    const unsigned wa = vw[k0 + 2 * x][c * VW + q4], wb = vw[k0 + 2 * x + 1][c * VW + q4];
+                    const unsigned t0 = __builtin_amdgcn_perm(wb, wa, 0x05010400u), t1 = __builtin_amdgcn_perm(wb, wa, 0x07030602u);
+                    vf[0][x] = pa_widen<PV, CT>(t0, false);
+                    vf[1][x] = pa_widen<PV, CT>(t0, true);
+                    if (VC > 2) {
+                      vf[2][x] = pa_widen<PV, CT>(t1, false);
+                      vf[3][x] = pa_widen<PV, CT>(t1, true);
+                    }
+                  }
                 }
+                // (the parts of P one after the other over the columns: products that follow each other do not wait for each other)
+#pragma unroll
+                for (int l = 0; l < PL; ++l)
+#pragma unroll
+                  for (int y = 0; y < 4; ++y) {
+                    if (4 * q4 + y < VC) {
+#pragma unroll
+                      for (int nt = 0; nt < NT; ++nt) acc[nt][c * VC + 4 * q4 + y] = pa_mfma16<PV>(vf[y], pf[nt][l], acc[nt][c * VC + 4 * q4 + y]);
+                    }
+                  }
               }
             }
           }
@@ -774,10 +788,15 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT)) void paged_attent
   }
 }
 
+template <int RT, int CT, int DP, int NT, int KT>
+static void pa_launch(const PagedAttn& a, unsigned blocks, hipStream_t stream) {
+  if (a.padding) hipLaunchKernelGGL((paged_attention_kernel<RT, CT, DP, NT, KT, true>), dim3(blocks), dim3(64 * PA_WAVES), 0, stream, a);
+  else hipLaunchKernelGGL((paged_attention_kernel<RT, CT, DP, NT, KT, false>), dim3(blocks), dim3(64 * PA_WAVES), 0, stream, a);
+}
 template <int RT, int CT, int DP, int NT>
 static void pa_launch(const PagedAttn& a, unsigned blocks, hipStream_t stream) {
-  if (a.padding) hipLaunchKernelGGL((paged_attention_kernel<RT, CT, DP, NT, true>), dim3(blocks), dim3(64 * PA_WAVES), 0, stream, a);
-  else hipLaunchKernelGGL((paged_attention_kernel<RT, CT, DP, NT, false>), dim3(blocks), dim3(64 * PA_WAVES), 0, stream, a);
+  a.workgroups ? pa_launch<RT, CT, DP, NT, pa_blocks(RT, CT, DP, NT, true)>(a, blocks, stream)
+               : pa_launch<RT, CT, DP, NT, pa_blocks(RT, CT, DP, NT, false)>(a, blocks, stream);
 }
 template <int RT, int CT>
 static void pa_launch(const PagedAttn& a, int tiles, unsigned blocks, hipStream_t stream) {

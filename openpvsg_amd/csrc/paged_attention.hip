@@ -24,11 +24,12 @@ static PaPlan pa_plan(const pvsg_kv_pages& p, int B, int T, int q_heads, int row
   s.row_groups = (rows + 16 * s.tiles - 1) / (16 * s.tiles);
   s.units = (long long)B * p.heads * s.row_groups;
   const long long capacity = (long long)table_width * p.page_size, longest = max_len > 0 && max_len < capacity ? max_len : capacity;
-  const bool f32_products = row_type == KV_F32 && (p.type == KV_F32 || p.type == KV_F16);
-  const int tile = PA_WAVES * (f32_products && p.dim > 32 ? 16 : 32);
-  const long long tiles = (longest + tile - 1) / tile;
-  if (tiles <= PA_SHORT || s.units * (capacity / tile + 1 + PA_PART) >= (1ll << 31)) return s;     // (the list is counted in 32 bits)
-  const long long room = 256 * pa_per_cu(p.dim, s.tiles), work = (s.units * (tiles + PA_PART) + PA_PART + PA_GRAIN - 1) / (PA_PART + PA_GRAIN);
+  const int dim = pa_dim(p.dim);
+  auto tile = [&](bool split) { return PA_WAVES * 16 * pa_blocks(row_type, p.type, dim, s.tiles, split); };
+  const int blocks = pa_blocks(row_type, p.type, dim, s.tiles, true), part = pa_part_cost(blocks);
+  if (longest <= (long long)PA_SHORT * tile(false) || s.units * (capacity / tile(true) + 1 + part) >= (1ll << 31)) return s;     // (the list is counted in 32 bits)
+  const long long tiles = (longest + tile(true) - 1) / tile(true);
+  const long long room = 256 * pa_per_cu(dim, s.tiles, blocks), work = (s.units * (tiles + part) + part + PA_GRAIN - 1) / (part + PA_GRAIN);
   s.workgroups = (int)(work < room ? work : room);
   const size_t rows_of = (size_t)2 * s.workgroups * 16 * s.tiles;
   s.part_o = rows_of * p.dim, s.part_ml = rows_of * 2;
