@@ -343,13 +343,15 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT, KT)) void paged_at
   } else {
     // every wave scans the lengths by itself: 64 lanes, `per` sequences each, the first four of them in registers
     const int lane = threadIdx.x & 63, per = (a.B + 63) / 64, b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B), capacity = a.width << a.page_shift;
+    auto entries = [&](int n) { return (unsigned)(PA_PART + tiles_of(n, capacity)); };
     int lens[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) lens[k] = b0 + k < b1 ? a.lens[b0 + k] : 0;
     unsigned mine = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) mine += b0 + k < b1 ? PA_PART + tiles_of(lens[k], capacity) : 0;
-    for (int i = b0 + 4; i < b1; ++i) mine += PA_PART + tiles_of(a.lens[i], capacity);
+    for (int k = 0; k < 4; ++k) mine += b0 + k < b1 ? entries(lens[k]) : 0;
+#pragma unroll 8
+    for (int i = b0 + 4; i < b1; ++i) mine += entries(a.lens[i]);
     mine *= each;
     const unsigned upto = pa_scan(mine);
     const unsigned total = __builtin_amdgcn_readlane(upto, 63);
@@ -359,22 +361,36 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT, KT)) void paged_at
     if (blockIdx.x >= used) return;
     left = share + (blockIdx.x < more ? 1 : 0);
     const int whose = __builtin_ctzll(__ballot(first < upto));      // the lane whose sequences the stretch begins in
-    unsigned before = upto - mine;
-    b = b0, len = lens[0];
-    bool found = false;
+    unsigned inside;
+    if (per <= 4) {
+      unsigned before = upto - mine;
+      b = b0, len = lens[0];
+      bool found = false;
 #pragma unroll
-    for (int k = 0; k < 3; ++k) {
-      const unsigned n = (PA_PART + tiles_of(lens[k], capacity)) * each;
-      found |= b0 + k >= b1 - 1 || first < before + n;
-      if (!found) before += n, b = b0 + k + 1, len = lens[k + 1];
+      for (int k = 0; k < 3; ++k) {
+        const unsigned n = entries(lens[k]) * each;
+        found |= b0 + k >= b1 - 1 || first < before + n;
+        if (!found) before += n, b = b0 + k + 1, len = lens[k + 1];
+      }
+      b = __builtin_amdgcn_readlane(b, whose), len = __builtin_amdgcn_readlane(len, whose);
+      inside = first - __builtin_amdgcn_readlane(before, whose);
+    } else {
+      // that lane's sequences, 64 at a time
+      unsigned before = __builtin_amdgcn_readlane(upto - mine, whose);
+      const int end = min((whose + 1) * per, a.B);
+      for (b = whose * per;; b += 64) {
+        const int mine_len = b + lane < end ? a.lens[b + lane] : 0;
+        const unsigned n = b + lane < end ? entries(mine_len) * each : 0, sum = pa_scan(n);
+        const unsigned long long here = __ballot(first < before + sum);
+        if (here) {                                                 // (in the last 64 at the latest)
+          const int l = __builtin_ctzll(here);
+          b += l, len = __builtin_amdgcn_readlane(mine_len, l), inside = first - before - __builtin_amdgcn_readlane(sum - n, l);
+          break;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
+        if (b + 64 >= end) return;                                  // never: the lane's sequences hold `first`
+      }
     }
-    while (!found && b < b1 - 1) {
-      const unsigned n = (PA_PART + tiles_of(len, capacity)) * each;
-      if (first < before + n) break;
-      before += n, len = a.lens[++b];
-    }
-    b = __builtin_amdgcn_readlane(b, whose), len = __builtin_amdgcn_readlane(len, whose);
-    const unsigned inside = first - __builtin_amdgcn_readlane(before, whose);
     const unsigned n = PA_PART + tiles_of(len, capacity);
     hr = inside / n, at = inside - hr * n;
   }

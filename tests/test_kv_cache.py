@@ -386,6 +386,20 @@ def test_attention_split_over_a_long_cache(hip_lib, row, pool, D):
 
 
 @gpu
+@pytest.mark.parametrize('B', (63, 64, 65, 129, 256, 257, 300, 1500, 4200))
+def test_attention_batches_of_every_size(hip_lib, B):
+    """the shares of a long batch: most sequences short, some long, some empty (each workgroup finds its share by a scan over the lengths)"""
+    from openpvsg_amd import ops
+    g = torch.Generator().manual_seed(B)
+    lens = (1 + 60 * torch.rand(B, generator=g) ** 3).int()
+    lens[torch.randint(0, B, (max(2, B // 50),), generator=g)] = 0
+    lens[torch.randint(0, B, (3,), generator=g)] = torch.tensor([1500, 2500, 1100], dtype=torch.int32)
+    lens[B - 1] = 1300
+    c = Cache(ops, lens.tolist(), 1, 16, 16, torch.float32, B)
+    check(ops, c, queries((B, 1, 2, 16), torch.float32, B))
+
+
+@gpu
 def test_attention_scale_and_large_logits(hip_lib):
     from openpvsg_amd import ops
     c = Cache(ops, [130, 64], 2, 64, 16, torch.float32, 3)
