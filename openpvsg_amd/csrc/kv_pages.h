@@ -115,6 +115,9 @@ __device__ __forceinline__ void kv_fault(int* faults, int bit) {
   if (faults) __hip_atomic_fetch_or(faults, bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// a launch of 256-thread workgroups holds fewer than 2^32 threads
+constexpr long long KV_MAX_BLOCKS = 1ll << 24;
+
 // the checks every entry point makes of its pool
 int kv_check_pages(const char* who, const pvsg_kv_pages* p, const int* table, long long table_stride, int table_width, const int* lens, int B);
 

@@ -65,7 +65,7 @@ constexpr bool pa_16bit(int row, int pool) { return row != KV_F32 || pool == KV_
 constexpr int pa_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 // 16-key blocks of a wave's tile.  f32 products take one key at a time, so that a block of theirs is work enough.  Of heads of up to 64
 // in 16 bits there is room for four beside the next tile's, and where the caches are long (`split`: the tiles are shared out) they
-// save waits for memory: 64 x 8192 x 8 heads of 64 int8 123 -> 112 us, 20 ragged ones of up to 3000 18.0 -> 15.6.  Short ones go two blocks at a time,
+// save waits for memory: 64 x 8192 x 8 heads of 64 int8 122 -> 109 us, 20 ragged ones of up to 3000 18.1 -> 15.7.  Short ones go two blocks at a time,
 // three workgroups to a CU: 100 of up to 900 positions 19.3 us, and 22.3 with four.
 constexpr int pa_blocks(int row, int pool, int dim, int tiles, bool split) {
   return pa_16bit(row, pool) ? (split && tiles == 1 && row != KV_F32 && dim <= 64 ? 4 : 2) : dim <= 32 ? 2 : 1;

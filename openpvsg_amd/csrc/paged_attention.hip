@@ -65,7 +65,7 @@ extern "C" int pvsg_paged_attention(const pvsg_kv_pages* pages, const void* q, l
   PVSG_REQUIRE(s.workgroups == 0 || (workspace && counters && (((uintptr_t)workspace & 15) | ((uintptr_t)counters & 3)) == 0),
                "pvsg_paged_attention: workspace %p and counters %p, %lld bytes are needed", workspace, static_cast<void*>(counters),
                (long long)(s.part_o + s.part_ml) * 4);
-  PVSG_REQUIRE(s.units < (1ll << 31), "pvsg_paged_attention: %lld parts are too many for one launch", s.units);
+  PVSG_REQUIRE(s.workgroups || s.units < KV_MAX_BLOCKS, "pvsg_paged_attention: %lld parts are too many for one launch", s.units);
   PagedAttn a{};
   a.p = *pages;
   a.q = static_cast<const unsigned char*>(q), a.out = static_cast<unsigned char*>(out);

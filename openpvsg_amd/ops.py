@@ -1725,8 +1725,8 @@ def kv_append(pages, k, v, table, lens, new_lens=None):
     8-bit pools: scale = max(max|row| * (1/448 or 1/127), 2^-126), code = round(row / scale), ties to even; a row with a NaN or infinity reads
     back as NaN.  Pages that are appended to belong to one sequence.  Page ids out of the pool: skipped, see page_fault_check."""
     k, v = _kv_rows(k, 'k', pages, pages.heads), _kv_rows(v, 'v', pages, pages.heads)
-    if pages.k.data_ptr() == pages.v.data_ptr():
-        raise RuntimeError('kv_append: the pool\'s k and v are the same memory')
+    if pages.k.data_ptr() == pages.v.data_ptr() or (pages.k_scale is not None and pages.k_scale.data_ptr() == pages.v_scale.data_ptr()):
+        raise RuntimeError('kv_append: the pool\'s k and v, or their scales, are the same memory')
     if k.shape != v.shape or k.dtype != v.dtype:
         raise RuntimeError('kv_append: k %s %s and v %s %s differ' % (tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
     if k.stride() != v.stride():
@@ -1791,7 +1791,7 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
     up to its own; with key_padding_mask (B, M) bool, True = ignored as in torch's attention, and positions from M on ignored too.
     A row that sees nothing (an empty sequence, a token past n, everything masked) is zero; what is masked never reaches a
     result, NaN and infinities included.  scale defaults to head_dim ** -0.5.  max_len: the longest cache to plan the split for, if
-    the table holds much more (longer ones are computed all the same).  out: (B, T, q_heads, head_dim), contiguous.
+    the table holds much more (longer ones are computed all the same).  out: (B, T, q_heads, head_dim), contiguous, apart from q.
     -> (B, T, q_heads, head_dim)"""
     q = _kv_rows(q, 'q', pages, None)
     B, T, HQ, D = q.shape
@@ -1817,6 +1817,9 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
     elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or \
             out.data_ptr() & 15 or out.requires_grad:
         raise RuntimeError('paged_attention: out must be a contiguous, 16-byte aligned %s tensor of shape %s on %s' % (q.dtype, tuple(q.shape), q.device))
+    elif out.data_ptr() < q.data_ptr() + (sum((n - 1) * s for n, s in zip(q.shape, q.stride())) + 1) * q.element_size() and \
+            q.data_ptr() < out.data_ptr() + out.numel() * out.element_size() and out.numel():
+        raise RuntimeError('paged_attention: out overlaps q')
     if mask is not None and mw == 0:
         return out.zero_()
     if B == 0 or T == 0:

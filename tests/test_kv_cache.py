@@ -177,6 +177,16 @@ def test_bad_calls_are_refused(hip_lib):
     assert append(B=0) == 0 and append(T=0) == 0 and read(length=0) == 0 and read(B=0) == 0 and attend(B=0) == 0 and attend(T=0) == 0
 
 
+def test_calls_past_one_launch_are_refused(hip_lib):
+    """a launch holds fewer than 2^32 threads: 2^24 workgroups of 256"""
+    p, one = pages_struct(dim=256, heads=1, page_stride=16 * 256, head_stride=16 * 256, slot_stride=256), ctypes.c_void_p(4096)
+    big = (1 << 27) + 8                                              # rows of 32 lanes
+    assert hip_lib.pvsg_kv_append(p, one, one, 0, 256, 256, 256, one, 2, 2, one, None, 1, big, None) == 1
+    assert hip_lib.pvsg_kv_read(p, one, one, 0, one, 2, 2, one, 1, 0, big, None) == 1
+    p = pages_struct(heads=1024)
+    assert hip_lib.pvsg_paged_attention(p, one, 64, 64, 64, one, 0, one, 2, 2, one, None, None, 0, 0, 65535, 1, 1024, 1.0, 1, 0, None, None, None) == 1
+
+
 def test_workspace_is_bounded_by_the_card(hip_lib):
     """none where every cache is a few tiles, and two parts for each of at most 1024 workgroups however long the caches are"""
     def f(B=1, T=1, HQ=4, row=0, width=1, longest=0, **kw):
@@ -515,6 +525,22 @@ def test_captured_and_eager_joins_give_the_same_bits(hip_lib, row, pool):
         fresh = torch.minimum(c.lens, torch.full_like(c.lens, T))
         want, tol = reference(q.cpu()[some], [c.rows[0][b] for b in some], [c.rows[1][b] for b in some], c.lens[some], fresh[some], None, True, D ** -0.5)
         assert bool(((out.cpu()[some].double() - want).abs() <= tol).all())
+
+
+@gpu
+def test_shared_memory_is_refused(hip_lib):
+    """scales that K and V share are not written, and the result does not go where the queries are read from"""
+    from openpvsg_amd import ops
+    f = lambda *s, dtype=torch.float32: torch.zeros(s, dtype=dtype, device='cuda')  # noqa: E731
+    table, lens, x, scales = f(3, 2, dtype=torch.int32), f(3, dtype=torch.int32), f(3, 1, 2, 32), f(4, 2, 8)
+    with pytest.raises(RuntimeError, match='same memory'):
+        ops.kv_append(ops.KVPages(f(4, 2, 8, 32, dtype=torch.int8), f(4, 2, 8, 32, dtype=torch.int8), scales, scales), x, x, table, lens)
+    p, both = ops.KVPages.empty(4, 2, 8, 32), f(6, 1, 4, 32)
+    for q, out in ((both[:3], both[:3]), (both[:3], both[2:5]), (both[2:5], both[:3]), (both[:, :, :2][:3], both.view(-1)[64:256].view(3, 1, 2, 32))):
+        with pytest.raises(RuntimeError, match='overlaps'):
+            ops.paged_attention(q, p, table, lens, out=out)
+    out = both[3:]
+    assert ops.paged_attention(both[:3], p, table, lens, out=out) is out
 
 
 @gpu
