@@ -1585,6 +1585,8 @@ _KV_SCALED = (torch.float8_e4m3fn, torch.int8)
 PAGED_ATTENTION_MAX_NEW = 32
 
 _page_faults = {}
+_attention_counters = {}
+_captured_counters = {}
 
 
 def _page_fault_word(device):
@@ -1592,8 +1594,11 @@ def _page_fault_word(device):
     if t is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError('KVPages: the first pool of a device cannot be made while a graph is captured')
-        # a blocking copy: the word is there for every stream
-        t = _page_faults[device.index] = torch.zeros(1, dtype=torch.int32).to(device)
+        # blocking copies: the words are there for every stream; ordinary tensors, whatever mode the first pool is made in
+        with torch.inference_mode(False):
+            t = _page_faults[device.index] = torch.zeros(1, dtype=torch.int32).to(device)
+            spare = torch.zeros((128, 1024), dtype=torch.int32).to(device)
+        _captured_counters[device.index] = (spare, iter(spare))     # (the whole stays: graphs hold its rows)
     return t
 
 
@@ -1767,15 +1772,13 @@ def kv_read(pages, table, lens, length, start=0, dtype=torch.float32):
     return tuple(out)
 
 
-_attention_counters = {}
-
-
 def _paged_attention_counters(device, stream):
     """Zeroed words by which the workgroups of a launch find out who joins a split row: one set for each stream, whose launches
-    follow each other and leave them zero.  A launch that is captured gets its own, cleared in the graph: replays may run beside
-    anything."""
+    follow each other and leave them zero.  A launch that is captured gets its own, since replays may run beside anything: one of 128 that
+    were cleared beforehand, and after those one that the graph clears (a kernel more: 17.4 us a replayed call where the others take 15)."""
     if torch._C._cuda_isCurrentStreamCapturing():
-        return torch.zeros(1024, dtype=torch.int32, device=torch.device('cuda', device))
+        t = next(_captured_counters[device][1], None)
+        return t if t is not None else torch.zeros(1024, dtype=torch.int32, device=torch.device('cuda', device))
     t = _attention_counters.get((device, stream))
     if t is None:
         t = _attention_counters[device, stream] = torch.zeros(1024, dtype=torch.int32).to(torch.device('cuda', device))

@@ -712,6 +712,46 @@ def test_steps_replay_from_graphs(hip_lib):
 
 
 @gpu
+def test_a_first_pool_made_in_inference_mode(hip_lib, monkeypatch):
+    """the fault word that it makes is one that a check outside that mode can clear"""
+    from openpvsg_amd import ops
+    monkeypatch.setattr(ops, '_page_faults', {})
+    monkeypatch.setattr(ops, '_captured_counters', {})
+    with torch.inference_mode():
+        pages = ops.KVPages.empty(2, 1, 8, 16)
+        table, lens = torch.full((1, 1), 2, dtype=torch.int32, device='cuda'), torch.ones(1, dtype=torch.int32, device='cuda')
+        ops.kv_append(pages, torch.ones(1, 1, 1, 16, device='cuda'), torch.ones(1, 1, 1, 16, device='cuda'), table, lens)
+    with pytest.raises(RuntimeError, match='kv_append met page ids'):
+        ops.page_fault_check()
+    ops.page_fault_check()
+    torch.cuda.synchronize()
+
+
+@gpu
+def test_captured_calls_beyond_the_cleared_counters(hip_lib, monkeypatch):
+    """the last set that was cleared beforehand, then sets that the graph clears; replays between eager calls"""
+    from openpvsg_amd import ops
+    c = Cache(ops, [3000, 700, 1900], 2, 64, 16, torch.float32, 5)
+    q = queries((3, 2, 4, 64), torch.float32, 5).cuda()
+    eager = ops.paged_attention(q, c.pages, c.dev_table, c.dev_lens)
+    spare, _ = ops._captured_counters[q.get_device()]
+    last = torch.zeros(1024, dtype=torch.int32).cuda()               # (lives as long as the graph)
+    monkeypatch.setitem(ops._captured_counters, q.get_device(), (spare, iter([last])))
+    torch.cuda.synchronize()
+    graph, outs = torch.cuda.CUDAGraph(), []
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            outs.append(ops.paged_attention(q, c.pages, c.dev_table, c.dev_lens))
+    for _ in range(4):
+        for o in outs:
+            o.fill_(7.0)
+        again = ops.paged_attention(q, c.pages, c.dev_table, c.dev_lens)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(bits(o), bits(eager)) for o in outs + [again])
+
+
+@gpu
 def test_another_stream(hip_lib):
     from openpvsg_amd import ops
     c = Cache(ops, [500, 3], 2, 64, 16, torch.bfloat16, 3)
