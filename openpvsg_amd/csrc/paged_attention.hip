@@ -29,6 +29,7 @@ static PaPlan pa_plan(const pvsg_kv_pages& p, int B, int T, int q_heads, int row
   const int blocks = pa_blocks(row_type, p.type, dim, s.tiles, true), part = pa_part_cost(blocks);
   if (longest <= (long long)PA_SHORT * tile(false) || s.units * (capacity / tile(true) + 1 + part) >= (1ll << 31)) return s;     // (the list is counted in 32 bits)
   const long long tiles = (longest + tile(true) - 1) / tile(true);
+  static_assert(256 * pa_per_cu(32, 1, 2) <= PVSG_PAGED_ATTENTION_COUNTERS, "a counter for each workgroup");
   const long long room = 256 * pa_per_cu(dim, s.tiles, blocks), work = (s.units * (tiles + part) + part + PA_GRAIN - 1) / (part + PA_GRAIN);
   s.workgroups = (int)(work < room ? work : room);
   const size_t rows_of = (size_t)2 * s.workgroups * 16 * s.tiles;
