@@ -323,6 +323,11 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT, KT)) void paged_at
   constexpr int KC = 16 / CB < DP / 4 ? 16 / CB : DP / 4, NK = DP / (4 * KC), KW = KC * CB / 4;
   constexpr int VE = DP / 16, VC = 16 / CB < VE ? 16 / CB : VE, NV = VE / VC, VB = VC * CB, VW = (VB + 3) / 4;
   constexpr int QN = M16 ? DP / 32 : DP / 4;                        // steps of 8 packed columns, or single columns
+  // f16 has no normal numbers below 2^-14 and nothing below 2^-25, and weights there count where the largest one's value does not.
+  // So m is held 15 below the maximum: weights of up to 2^15, whose two f16 parts hold 22 bits down to 2^-29 of the largest one and
+  // 2^-40 of it below.  O and l have the same factor, and (m, l, O) mean what they do without it.  (Maxima so large that their
+  // f32 is not exact to a few units can make a weight infinite: such rows are computed again.)
+  constexpr float LIFT = M16 && PV == KV_F16 ? 15.f : 0.f;
   static_assert(!M16 || KC % 8 == 0, "16-bit products take 8 columns a lane");
 
   __shared__ int s_page[PA_CHUNK / 8 + 1];
@@ -620,7 +625,7 @@ __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT, KT)) void paged_at
           }
 #pragma unroll
           for (int k = 0; k < KT * 4; ++k) top = fmaxf(top, z[k]);
-          top = fmaxf(pa_max4(top), mrow[nt]);
+          top = fmaxf(pa_max4(top) - LIFT, mrow[nt]);
           const float ref = top == -INFINITY ? 0.f : top;             // a row that has seen nothing yet
           if (__any(top > mrow[nt])) {
             const float shrink = __builtin_amdgcn_exp2f(mrow[nt] - ref);
