@@ -15,10 +15,12 @@
 // no cache is longer than a few tiles there is nothing to even out, and each has a workgroup of its own and no join.
 //
 // Rounding: 16-bit rows multiply in their own type, exact products in f32 sums; 8-bit codes convert to it exactly and their
-// scales multiply S and P in f32.  P goes to the matrix cores as a 16-bit high part plus a 16-bit rest (one part alone adds an error as
-// large as the rounding of the result itself).  f32 rows over a bf16 or 8-bit pool go as three bf16 parts, which hold all
-// 24 bits, and so does their P: three 16-bit products take an eighth of the matrix cores' time that the f32 ones would.  f32 rows over a
-// f32 or f16 pool run on the f32 products.
+// scales multiply S and P in f32.  P goes to the matrix cores with the bits that f32 has: as three bf16 parts over a bf16 or 8-bit pool,
+// as two f16 parts over a f16 one (see LIFT).  One part alone adds an error as large as the rounding of the result itself; two of bf16
+// hold 16 bits, which shows where values cancel, and save little (100 x up to 5000 x 4 x 128 e4m3, 32 new tokens: 77.4 us, three parts
+// 79.7; 64 x 8192 x 8 heads of 64 int8 110.8 and 116.7; 8 x 65536 bf16 361 both).  f32 rows over a bf16 or 8-bit pool go as three bf16 parts too.  At
+// the matrix cores' peak three 16-bit products take 3/16 of the time that the f32 ones would.  f32 rows over a f32 or f16 pool run on the f32
+// products.
 //
 // Measured: 8 x 65536 x 8 key heads of 128 bf16 359 us, 5.95 TB/s, bound by HBM; 100 ragged caches of up to 900 x 4 x 128 f32 48 us,
 // 3.85 TB/s: a stretch takes 5 us to its first keys (lengths, scan, page ids, queries: waits for memory that depend on each other)
@@ -316,7 +318,7 @@ template <int RT, int CT, int DP, int NT, int KT, bool PADDED>
 __global__ __launch_bounds__(64 * PA_WAVES, pa_per_cu(DP, NT, KT)) void paged_attention_kernel(const PagedAttn) {
   constexpr bool M16 = pa_16bit(RT, CT);
   constexpr int QK = RT == KV_F16 ? KV_F16 : KV_BF16, PV = CT == KV_F16 ? KV_F16 : KV_BF16;      // operand types of the 16-bit products
-  constexpr int QL = RT == KV_F32 ? 3 : 1, PL = RT == KV_F32 ? 3 : 2;
+  constexpr int QL = RT == KV_F32 ? 3 : 1, PL = PV == KV_BF16 ? 3 : 2;
   constexpr int CB = kv_bytes(CT), RB = kv_bytes(RT);
   constexpr int KEYS = 16 * KT, PA_PART = pa_part_cost(KT);           // a wave's tile is KT blocks of 16 keys
   // keys: chunk i of a lane in 16-lane group g is columns i*4*KC + KC*g ...; values: column c*16*VC + VC*m + e for lane m

@@ -52,3 +52,56 @@ def test_small_f16_weights_behind_a_dominant_key(hip_lib, D, above):
                 tol = (rel + 2.0 ** -22) * size + 2.0 ** -40 * every + torch.finfo(torch.float16).eps / 2 * want.abs() + 2.0 ** -25
                 err = (got[b, t, j] - want).abs()
                 assert bool((err <= tol).all()), (b, t, j, 'worst %.3g of its tolerance' % float((err / tol).max()))
+
+
+def cancelling(n, H, D, pool, g):
+    """n keys whose weights are known to a few units of f32 (one column of k, the rest zero; exact logits in [-1, 0]) and values that
+    cancel under them: the last keys' take back what the ones before leave, so what is left of a result is the weights' own error"""
+    z = -(torch.randint(0, 17, (n, H), generator=g) / 16.0)
+    z[0] = 0.0
+    w = torch.exp(z.double())
+    v = torch.where(torch.rand((n, H, D), generator=g) < 0.5, -1.0, 1.0) * (1.0 + torch.randint(0, 8, (n, H, D), generator=g) / 8.0)
+    scaled = pool == torch.float8_e4m3fn
+    scale = torch.ones(n, H)
+    for i in range(n - (6 if scaled else 3), n):
+        left = -(w[:i, :, None] * v[:i].double() * scale[:i, :, None]).sum(0) / w[i, :, None]
+        if scaled:
+            scale[i] = 2.0 ** torch.ceil(torch.log2(left.abs().amax(-1))).float() / 256.0
+        v[i] = (left / scale[i, :, None]).float().to(pool).float()
+    k = torch.zeros(n, H, D)
+    k[..., 0] = z
+    return k, v, scale, w
+
+
+@gpu
+@pytest.mark.parametrize('row,pool', ((torch.bfloat16, torch.bfloat16), (torch.bfloat16, torch.float8_e4m3fn), (torch.float16, torch.float8_e4m3fn),
+                                      (torch.float16, torch.float16), (torch.float32, torch.bfloat16)), ids=lambda t: str(t)[6:])
+def test_weights_hold_the_bits_of_f32(hip_lib, row, pool):
+    from openpvsg_amd import ops
+    B, n, H, D = 60, 12, 4, 16
+    c = Cache(ops, [n] * B, H, D, 16, pool, 1)
+    g = torch.Generator().manual_seed(3)
+    per = [cancelling(n, H, D, pool, g) for _ in range(B)]
+    at = c.table[:, 0].long().cuda()
+
+    def put(codes, x):
+        x = x.transpose(1, 2).to(pool)
+        if pool == torch.float8_e4m3fn:
+            codes, x = codes.view(torch.uint8), x.view(torch.uint8)
+        codes[at, :, :n] = x.cuda()
+    put(c.pages.k, torch.stack([p[0] for p in per]))
+    put(c.pages.v, torch.stack([p[1] for p in per]))
+    if pool == torch.float8_e4m3fn:
+        c.pages.k_scale[at, :, :n] = 1.0
+        c.pages.v_scale[at, :, :n] = torch.stack([p[2] for p in per]).transpose(1, 2).cuda()
+    q = torch.zeros(B, 1, H, D, dtype=row)
+    q[..., 0] = 1.0
+    got = ops.paged_attention(q.cuda(), c.pages, c.dev_table, c.dev_lens, scale=1.0).cpu().double()[:, 0]
+    for b, (k, v, scale, w) in enumerate(per):
+        x = v.double() * scale.double()[..., None]
+        want = (w[..., None] * x).sum(0) / w.sum(0)[:, None]
+        # what f32 gives: z * log2(e) and its rounding, |z| <= 1: 3 * 2^-24; exp2 2^-23; three parts or two of f16 2^-22; the product with a scale
+        # 2^-24; the sums over at most 16 keys, three parts each, and over the four waves: 16 * 2^-24.  One rounding of the result.
+        tol = 26 * 2.0 ** -24 * (w[..., None] * x.abs()).sum(0) / w.sum(0)[:, None] + torch.finfo(row).eps / 2 * want.abs() + (2.0 ** -25 if row == torch.float16 else 0.0)
+        err = (got[b] - want).abs()
+        assert bool((err <= tol).all()), (b, 'worst %.3g of its tolerance' % float((err / tol).max()))
