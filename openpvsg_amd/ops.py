@@ -1604,13 +1604,18 @@ def _page_fault_word(device):
 
 def page_fault_check(device=None):
     """Raise RuntimeError if a page table or a length sent kv_append / kv_read / paged_attention outside a pool or a table since the
-    last check, on `device` (default: the current one).  Synchronises.  What they skipped was not written, read as zeros, or
-    was not attended to."""
+    last check, on `device` (default: the current one).  Waits for the whole device, whatever stream the calls went to.  What they skipped was
+    not written, read as zeros, or was not attended to."""
     d = torch.device('cuda' if device is None else device)
-    t = _page_faults.get(d.index if d.index is not None else torch.cuda.current_device())
-    bits = int(t.item()) if t is not None else 0
+    index = d.index if d.index is not None else torch.cuda.current_device()
+    t = _page_faults.get(index)
+    if t is None:
+        return
+    torch.cuda.synchronize(index)                                   # torch's own streams do not wait for each other
+    bits = int(t.item())
     if bits:
         t.zero_()
+        torch.cuda.synchronize(index)                               # a later call on any stream finds it cleared
         who = [n for i, n in enumerate(('kv_append', 'kv_read', 'paged_attention')) if bits >> i & 1]
         raise RuntimeError('%s met page ids outside the pool, or lengths past the page table: those positions were skipped'
                            % ', '.join(who))
