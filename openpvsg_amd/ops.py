@@ -1621,13 +1621,32 @@ def page_fault_check(device=None):
                            % ', '.join(who))
 
 
+def _rows_meet(delta, axes, size):
+    """whether the rows of `size` at sum(i * stride) over `axes` = ((stride, count), ...), each axis' stride no less than what the ones
+    behind it span, share memory with the same rows shifted by `delta`"""
+    if not axes:
+        return abs(delta) < size
+    stride, n = axes[0]
+    near = delta // stride                                          # what the inner axes differ by is less than one stride
+    return any(_rows_meet(delta - i * stride, axes[1:], size) for i in (near, near + 1) if -n < i < n)
+
+
+def _rows_touch(base, axes, size, lo, hi):
+    """whether one of such rows from `base` on shares memory with lo .. hi - 1"""
+    at = base
+    for stride, n in axes:                                          # the last row that begins before hi
+        at += max(0, min(n - 1, (hi - 1 - at) // stride)) * stride
+    return lo < at + size and at < hi
+
+
 class KVPages:
     """A pool of key / value pages: k, v (num_pages, heads, page_size, head_dim), any strides with a dense last axis (a pool
     laid out (num_pages, page_size, heads, head_dim) is passed as `.transpose(1, 2)`), float32, bfloat16, float16, or 8-bit
     (float8_e4m3fn, int8) with a float32 scale per row, k_scale / v_scale (num_pages, heads, page_size), contiguous.
     Slots hold x, 8-bit ones x / scale.  The pool is written in place by `kv_append`; its tensors stay the caller's."""
 
-    __slots__ = ('k', 'v', 'k_scale', 'v_scale', 'dtype', 'device', 'index', 'num_pages', 'heads', 'page_size', 'head_dim', '_struct')
+    __slots__ = ('k', 'v', 'k_scale', 'v_scale', 'dtype', 'device', 'index', 'num_pages', 'heads', 'page_size', 'head_dim', '_struct',
+                 '_axes', '_spans', '_shared')
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         for n, t in (('k', k), ('v', v)):
@@ -1661,6 +1680,14 @@ class KVPages:
             for n, t in (('k_scale', k_scale), ('v_scale', v_scale)):
                 if _chk(t, 'KVPages: ' + n).data_ptr() != t.data_ptr() or tuple(t.shape) != (P, H, S) or t.device != k.device or t.data_ptr() & 15:
                     raise RuntimeError('KVPages: %s must be contiguous (num_pages, heads, page_size) on the pool\'s device' % n)
+        # memory that an append writes: axes of the code rows in bytes, outermost first; where each tensor lies; whether one of them meets another
+        size = k.element_size()
+        self._axes = tuple(sorted(((stride * size, n) for stride, n in ((sp, P), (sh, H), (ss, S)) if n > 1), reverse=True))
+        at = k.data_ptr(), v.data_ptr()
+        codes, scales = [(a, a + extent * size) for a in at], [(t.data_ptr(), t.data_ptr() + 4 * t.numel()) for t in (k_scale, v_scale) if scaled]
+        self._spans = tuple(codes + scales)
+        self._shared = _rows_meet(at[1] - at[0], self._axes, D * size) or any(_rows_touch(a, self._axes, D * size, *t) for a in at for t in scales) or \
+            (scaled and scales[0][0] < scales[1][1] and scales[1][0] < scales[0][1])
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.dtype, self.device, self.index = k.dtype, k.device, k.get_device()
         self.num_pages, self.heads, self.page_size, self.head_dim = P, H, S, D
@@ -1726,6 +1753,21 @@ def _kv_rows(t, name, pages, heads):
     return t if _kv_aligned(t) else t.clone(memory_format=torch.contiguous_format)
 
 
+def _kv_meets(out, pages, *others):
+    """whether the dense tensor `out` shares memory with the pool or another input"""
+    lo = out.data_ptr()
+    hi = lo + out.numel() * out.element_size()
+    size = pages.head_dim * pages.k.element_size()
+    if any(_rows_touch(a, pages._axes, size, lo, hi) for a, _ in pages._spans[:2]) or any(lo < b and a < hi for a, b in pages._spans[2:]):
+        return True
+    for t in others:
+        if t is not None and t.numel():
+            a = t.data_ptr()
+            if lo < a + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() and a < hi:
+                return True
+    return False
+
+
 def kv_append(pages, k, v, table, lens, new_lens=None):
     """Write new rows into the pool, rounding or quantising them to its type (one pass, in place).
 
@@ -1733,10 +1775,11 @@ def kv_append(pages, k, v, table, lens, new_lens=None):
     table[b, p // page_size]; lens (B,) int32: positions of each sequence INCLUDING the new ones.  Of sequence b's T rows the first
     n = min(T, lens[b], new_lens[b]) are written, at positions lens[b] - n ..; new_lens (B,) int32 defaults to T everywhere.
     8-bit pools: scale = max(max|row| * (1/448 or 1/127), 2^-126), code = round(row / scale), ties to even; a row with a NaN or infinity reads
-    back as NaN.  Pages that are appended to belong to one sequence.  Page ids out of the pool: skipped, see page_fault_check."""
+    back as NaN.  Pages that are appended to belong to one sequence.  Rows that are views of the pool count as they are before the call
+    (they are copied first).  Page ids out of the pool: skipped, see page_fault_check."""
     k, v = _kv_rows(k, 'k', pages, pages.heads), _kv_rows(v, 'v', pages, pages.heads)
-    if pages.k.data_ptr() == pages.v.data_ptr() or (pages.k_scale is not None and pages.k_scale.data_ptr() == pages.v_scale.data_ptr()):
-        raise RuntimeError('kv_append: the pool\'s k and v, or their scales, are the same memory')
+    if pages._shared:
+        raise RuntimeError('kv_append: the pool\'s k and v, or their scales, are the same memory in part')
     if k.shape != v.shape or k.dtype != v.dtype:
         raise RuntimeError('kv_append: k %s %s and v %s %s differ' % (tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
     if k.stride() != v.stride():
@@ -1748,8 +1791,16 @@ def kv_append(pages, k, v, table, lens, new_lens=None):
     if B == 0 or T == 0:
         return pages
     sb, st, sh, _ = k.stride()
+    span = ((B - 1) * sb + (T - 1) * st + (k.shape[2] - 1) * sh + k.shape[3]) * k.element_size()
+    a, b = k.data_ptr(), v.data_ptr()
+    for lo, hi in pages._spans:
+        if (a < hi and lo < a + span) or (b < hi and lo < b + span):   # rows that lie in the pool: read before anything is written
+            k, v = k.clone(memory_format=torch.contiguous_format), v.clone(memory_format=torch.contiguous_format)
+            sb, st, sh, _ = k.stride()
+            a, b = k.data_ptr(), v.data_ptr()
+            break
     with _on(pages.device):
-        _lib.call('pvsg_kv_append', pages._struct, k.data_ptr(), v.data_ptr(), _KV_ROW_TYPES[k.dtype], sb, st, sh, table.data_ptr(), row,
+        _lib.call('pvsg_kv_append', pages._struct, a, b, _KV_ROW_TYPES[k.dtype], sb, st, sh, table.data_ptr(), row,
                   width, lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, B, T,
                   _stream_ptr())
     return pages
@@ -1799,7 +1850,7 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
     up to its own; with key_padding_mask (B, M) bool, True = ignored as in torch's attention, and positions from M on ignored too.
     A row that sees nothing (an empty sequence, a token past n, everything masked) is zero; what is masked never reaches a
     result, NaN and infinities included.  scale defaults to head_dim ** -0.5.  max_len: the longest cache to plan the split for, if
-    the table holds much more (longer ones are computed all the same).  out: (B, T, q_heads, head_dim), contiguous, apart from q.
+    the table holds much more (longer ones are computed all the same).  out: (B, T, q_heads, head_dim), contiguous, apart from every input.
     -> (B, T, q_heads, head_dim)"""
     q = _kv_rows(q, 'q', pages, None)
     B, T, HQ, D = q.shape
@@ -1828,6 +1879,8 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
     elif out.data_ptr() < q.data_ptr() + (sum((n - 1) * s for n, s in zip(q.shape, q.stride())) + 1) * q.element_size() and \
             q.data_ptr() < out.data_ptr() + out.numel() * out.element_size() and out.numel():
         raise RuntimeError('paged_attention: out overlaps q')
+    elif out.numel() and _kv_meets(out, pages, table, lens, new_lens, mask):
+        raise RuntimeError('paged_attention: out overlaps the pool, the table, the lengths or the mask')
     if mask is not None and mw == 0:
         return out.zero_()
     if B == 0 or T == 0:

@@ -1,8 +1,36 @@
 """Paged cache: calls that must be reported or refused, or whose memory must stay what it was."""
+import itertools
+import random
+
 import pytest
 import torch
 
 gpu = pytest.mark.gpu
+
+
+def test_overlap_of_strided_rows_is_exact():
+    """both statements against the rows written out, over random nested axes with and without gaps"""
+    from openpvsg_amd import ops
+    r = random.Random(1)
+    met = touched = 0
+    for _ in range(3000):
+        size, axes, extent = r.choice((1, 2, 5)), [], 0
+        extent = size
+        for _ in range(r.randint(0, 3)):
+            stride, n = extent + r.choice((0, 0, 1, 3, 9)), r.randint(2, 4)
+            axes.insert(0, (stride, n))
+            extent += stride * (n - 1)
+        rows = [sum(i * s for i, (s, _) in zip(at, axes)) for at in itertools.product(*(range(n) for _, n in axes))]
+        mine = {x + d for x in rows for d in range(size)}
+        delta = r.randint(-extent - 3, extent + 3)
+        want = bool(mine & {x + delta for x in mine})
+        assert ops._rows_meet(delta, tuple(axes), size) == want, (delta, axes, size)
+        lo = r.randint(-3, extent + 3)
+        hi = lo + r.randint(1, 6)
+        want_touch = bool({x + 100 for x in mine} & set(range(100 + lo, 100 + hi)))
+        assert ops._rows_touch(100, tuple(axes), size, 100 + lo, 100 + hi) == want_touch, (lo, hi, axes, size)
+        met, touched = met + want, touched + want_touch
+    assert 300 < met < 2700 and 300 < touched < 2700
 
 
 @gpu
@@ -23,4 +51,79 @@ def test_a_fault_on_another_stream_is_reported(hip_lib):
     with pytest.raises(RuntimeError, match='kv_append met'):
         ops.page_fault_check()
     ops.page_fault_check()                                          # reported once
+    torch.cuda.synchronize()
+
+
+@gpu
+@pytest.mark.parametrize('dtype', (torch.float32, torch.int8), ids=str)
+def test_pools_that_share_memory(hip_lib, dtype):
+    """k and v a page, a slot or half a row apart are not appended to; interleaved ones, which share none, are"""
+    from openpvsg_amd import ops
+    P, H, S, D = 6, 2, 8, 32
+    table, lens, x = torch.arange(4, dtype=torch.int32, device='cuda').view(1, 4), torch.tensor([9], dtype=torch.int32, device='cuda'), torch.randn(1, 9, H, D, device='cuda')
+    scales = [torch.zeros(P, H, S, device='cuda') for _ in range(2)] if dtype == torch.int8 else []
+    flat = torch.zeros(4 * P * H * S * D, dtype=dtype, device='cuda')
+    for apart in (0, 16, D, S * D, H * S * D, (P - 1) * H * S * D):
+        k, v = (flat[at:at + P * H * S * D].view(P, H, S, D) for at in (0, apart))
+        with pytest.raises(RuntimeError, match='same memory'):
+            ops.kv_append(ops.KVPages(k, v, *scales), x, x, table, lens)
+    if scales:
+        both = torch.zeros(P * H * S + 16, device='cuda')
+        a, b = both[:P * H * S].view(P, H, S), both[16:].view(P, H, S)
+        with pytest.raises(RuntimeError, match='same memory'):
+            ops.kv_append(ops.KVPages(flat[:P * H * S * D].view(P, H, S, D), flat[P * H * S * D:2 * P * H * S * D].view(P, H, S, D), a, b), x, x, table, lens)
+        with pytest.raises(RuntimeError, match='same memory'):       # a scale inside the codes
+            ops.kv_append(ops.KVPages(flat[:P * H * S * D].view(P, H, S, D), flat[P * H * S * D:2 * P * H * S * D].view(P, H, S, D),
+                                      flat[:P * H * S * 4].view(torch.float32).view(P, H, S), scales[1]), x, x, table, lens)
+    for split in (flat[:2 * P * H * S * D].view(P, 2, H, S, D).unbind(1), flat[:2 * P * H * S * D].view(P, H, S, 2, D).unbind(3),
+                  flat[:2 * P * H * S * D].view(P, H, S, 2 * D).chunk(2, 3)):
+        pages = ops.KVPages(*split, *scales)
+        ops.kv_append(pages, x, 2 * x, table, lens)
+        k, v = ops.kv_read(pages, table, lens, 9)
+        assert float((v - 2 * k).abs().max()) <= 1e-6 and float((k - x).abs().max()) <= (0.0 if dtype == torch.float32 else 0.03)
+    torch.cuda.synchronize()
+
+
+@gpu
+def test_rows_that_lie_in_the_pool_count_as_they_were(hip_lib):
+    """a sequence's rows moved by one slot, within its own pages: each of them is read before any is written"""
+    from openpvsg_amd import ops
+    P, H, S, D = 8, 2, 16, 64
+    for dtype in (torch.float32, torch.bfloat16):
+        pages = ops.KVPages.empty(P, H, S, D, dtype=dtype)
+        table = torch.arange(P, dtype=torch.int32, device='cuda').view(P, 1)
+        pages.k.copy_(torch.randn(P, H, S, D, device='cuda')), pages.v.copy_(torch.randn(P, H, S, D, device='cuda'))
+        k, v = pages.k.clone(), pages.v.clone()
+        lens = torch.full((P,), S, dtype=torch.int32, device='cuda')
+        ops.kv_append(pages, pages.k.transpose(1, 2)[:, :-1], pages.v.transpose(1, 2)[:, :-1], table, lens)
+        for now, was in ((pages.k, k), (pages.v, v)):
+            assert torch.equal(now[:, :, 1:], was[:, :, :-1]) and torch.equal(now[:, :, 0], was[:, :, 0])
+        # both tensors from the same one's pages
+        ops.kv_append(pages, pages.v.transpose(1, 2)[:, :4], pages.v.transpose(1, 2)[:, :4], table, lens)
+        assert torch.equal(pages.k[:, :, -4:], pages.v[:, :, -4:]) and torch.equal(pages.k[:, :, 1:12], k[:, :, :11])
+    torch.cuda.synchronize()
+
+
+@gpu
+def test_out_may_not_lie_in_an_input(hip_lib):
+    from openpvsg_amd import ops
+    P, H, S, D = 6, 2, 8, 32
+    arena = torch.zeros(P, 3, H, S, D, device='cuda')
+    pages = ops.KVPages(arena[:, 0], arena[:, 1])
+    ints = torch.zeros(4 * 2 * H * D, dtype=torch.int32, device='cuda')
+    lens, q = torch.full((4,), 8, dtype=torch.int32, device='cuda'), torch.randn(4, 1, 2 * H, D, device='cuda')
+    table = torch.arange(4, dtype=torch.int32, device='cuda').view(4, 1)
+    mask = torch.zeros(4, 8, dtype=torch.bool, device='cuda')
+    n = q.numel()
+    want = ops.paged_attention(q, pages, table, lens, key_padding_mask=mask)
+    for out in (arena.view(-1)[:n], arena[3, 1].reshape(-1)[:n], arena.view(-1)[H * S * D * 5 - 16:][:n]):
+        with pytest.raises(RuntimeError, match='out overlaps the pool'):
+            ops.paged_attention(q, pages, table, lens, out=out.view(q.shape))
+    as_float = ints.view(torch.float32)
+    for kw in (dict(table=ints[:4].view(4, 1)), dict(lens=ints[-4:]), dict(new_lens=ints[:4]), dict(key_padding_mask=ints.view(torch.bool)[:32].view(4, 8))):
+        with pytest.raises(RuntimeError, match='out overlaps the pool'):
+            ops.paged_attention(q, pages, kw.pop('table', table), kw.pop('lens', lens), out=as_float[:n].view(q.shape), **kw)
+    out = arena[2, 2].reshape(-1)[:n].view(q.shape)                  # between the pool's rows
+    assert out.data_ptr() == arena[2, 2].data_ptr()
+    assert ops.paged_attention(q, pages, table, lens, key_padding_mask=mask, out=out) is out and torch.equal(out, want)
     torch.cuda.synchronize()
