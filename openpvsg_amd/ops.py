@@ -1643,7 +1643,8 @@ class KVPages:
     """A pool of key / value pages: k, v (num_pages, heads, page_size, head_dim), any strides with a dense last axis (a pool
     laid out (num_pages, page_size, heads, head_dim) is passed as `.transpose(1, 2)`), float32, bfloat16, float16, or 8-bit
     (float8_e4m3fn, int8) with a float32 scale per row, k_scale / v_scale (num_pages, heads, page_size), contiguous.
-    Slots hold x, 8-bit ones x / scale.  The pool is written in place by `kv_append`; its tensors stay the caller's."""
+    Slots hold x, 8-bit ones x / scale.  The pool is written in place by `kv_append`; its tensors stay the caller's.  A pool's tensors are
+    fixed: for others (a larger pool) make another KVPages."""
 
     __slots__ = ('k', 'v', 'k_scale', 'v_scale', 'dtype', 'device', 'index', 'num_pages', 'heads', 'page_size', 'head_dim', '_struct',
                  '_axes', '_spans', '_shared')
@@ -1694,6 +1695,15 @@ class KVPages:
         self._struct = _lib.KvPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if scaled else None,
                                     v_scale.data_ptr() if scaled else None, sp, sh, ss, H * S, S, P, H, S, D,
                                     _KV_TYPES[k.dtype], _page_fault_word(k.device).data_ptr())
+
+    def __setattr__(self, name, value):
+        # the kernels go by the addresses taken when the pool was made, and its tensors are kept alive for them
+        if hasattr(self, '_struct'):
+            raise AttributeError('KVPages: %s is fixed once the pool is made; make another KVPages' % name)
+        object.__setattr__(self, name, value)
+
+    def __delattr__(self, name):
+        raise AttributeError('KVPages: %s is fixed once the pool is made' % name)
 
     @classmethod
     def empty(cls, num_pages, heads, page_size, head_dim, dtype=torch.float32, device='cuda'):

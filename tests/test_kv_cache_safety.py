@@ -33,6 +33,20 @@ def test_overlap_of_strided_rows_is_exact():
     assert 300 < met < 2700 and 300 < touched < 2700
 
 
+def test_a_pools_tensors_are_fixed():
+    """a replaced tensor would be freed while the kernels go on writing to its address"""
+    from openpvsg_amd import _lib, ops
+    pages = ops.KVPages.__new__(ops.KVPages)
+    pages.k = pages.v = torch.zeros(2, 1, 8, 16)                    # as in the making
+    pages._struct = _lib.KvPages()
+    for name in ('k', 'v', 'k_scale', 'num_pages', '_struct'):
+        with pytest.raises(AttributeError, match='fixed'):
+            setattr(pages, name, torch.ones(4, 1, 8, 16))
+    with pytest.raises(AttributeError, match='fixed'):
+        del pages.k
+    assert pages.k.shape == (2, 1, 8, 16)
+
+
 @gpu
 def test_a_fault_on_another_stream_is_reported(hip_lib):
     """the check runs on the default stream while the faulting call still waits in another one's queue"""
