@@ -10,6 +10,7 @@ import os
 import weakref
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 
@@ -1621,6 +1622,12 @@ def page_fault_check(device=None):
                            % ', '.join(who))
 
 
+def _refuse_tangent(t, name):
+    """A dual tensor of forward-mode differentiation does not require a gradient: its tangent would be dropped without a word."""
+    if _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError('%s carries a forward-mode tangent: the paged cache is not differentiable' % name)
+
+
 def _rows_meet(delta, axes, size):
     """whether the rows of `size` at sum(i * stride) over `axes` = ((stride, count), ...), each axis' stride no less than what the ones
     behind it span, share memory with the same rows shifted by `delta`"""
@@ -1659,6 +1666,7 @@ class KVPages:
                 raise RuntimeError('KVPages: %s is %s; pools are float32, bfloat16, float16, float8_e4m3fn or int8' % (n, t.dtype))
             if t.requires_grad:
                 raise RuntimeError('KVPages: %s requires a gradient; the pool is written in place, without autograd' % n)
+            _refuse_tangent(t, 'KVPages: ' + n)
         if k.shape != v.shape or k.dtype != v.dtype or k.device != v.device or k.stride() != v.stride():
             raise RuntimeError('KVPages: k and v differ in shape, strides, dtype or device')
         P, H, S, D = k.shape
@@ -1681,6 +1689,9 @@ class KVPages:
             for n, t in (('k_scale', k_scale), ('v_scale', v_scale)):
                 if _chk(t, 'KVPages: ' + n).data_ptr() != t.data_ptr() or tuple(t.shape) != (P, H, S) or t.device != k.device or t.data_ptr() & 15:
                     raise RuntimeError('KVPages: %s must be contiguous (num_pages, heads, page_size) on the pool\'s device' % n)
+                if t.requires_grad:
+                    raise RuntimeError('KVPages: %s requires a gradient; the pool is written in place, without autograd' % n)
+                _refuse_tangent(t, 'KVPages: ' + n)
         # memory that an append writes: axes of the code rows in bytes, outermost first; where each tensor lies; whether one of them meets another
         size = k.element_size()
         self._axes = tuple(sorted(((stride * size, n) for stride, n in ((sp, P), (sh, H), (ss, S)) if n > 1), reverse=True))
@@ -1755,6 +1766,7 @@ def _kv_rows(t, name, pages, heads):
         raise RuntimeError('%s: %d heads of %d over a pool of %d heads of %d' % (name, H, D, pages.heads, pages.head_dim))
     if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError('%s requires a gradient: the paged cache is forward only (call it under torch.no_grad())' % name)
+    _refuse_tangent(t, name)
     if B > 65535:
         raise RuntimeError('%s: %d sequences (at most 65535)' % (name, B))
     if _kv_aligned(t):

@@ -47,6 +47,18 @@ def test_a_pools_tensors_are_fixed():
     assert pages.k.shape == (2, 1, 8, 16)
 
 
+def test_a_tangent_is_seen():
+    from torch.autograd import forward_ad
+
+    from openpvsg_amd import ops
+    x = torch.randn(3)
+    ops._refuse_tangent(x, 'x')
+    with forward_ad.dual_level():
+        ops._refuse_tangent(x, 'x')
+        with pytest.raises(RuntimeError, match='x carries a forward-mode tangent'):
+            ops._refuse_tangent(forward_ad.make_dual(x, torch.ones(3)), 'x')
+
+
 @gpu
 def test_a_fault_on_another_stream_is_reported(hip_lib):
     """the check runs on the default stream while the faulting call still waits in another one's queue"""
@@ -140,4 +152,30 @@ def test_out_may_not_lie_in_an_input(hip_lib):
     out = arena[2, 2].reshape(-1)[:n].view(q.shape)                  # between the pool's rows
     assert out.data_ptr() == arena[2, 2].data_ptr()
     assert ops.paged_attention(q, pages, table, lens, key_padding_mask=mask, out=out) is out and torch.equal(out, want)
+    torch.cuda.synchronize()
+
+
+@gpu
+def test_derivatives_are_refused(hip_lib):
+    """rows, pools and scales whose gradient or tangent would be dropped"""
+    from torch.autograd import forward_ad
+
+    from openpvsg_amd import ops
+    pages = ops.KVPages.empty(4, 2, 8, 32)
+    table, lens = torch.arange(4, dtype=torch.int32, device='cuda').view(2, 2), torch.full((2,), 3, dtype=torch.int32, device='cuda')
+    x, q = torch.ones(2, 3, 2, 32, device='cuda'), torch.ones(2, 3, 4, 32, device='cuda')
+    code, scale = torch.zeros(4, 2, 8, 32, dtype=torch.int8, device='cuda'), torch.ones(4, 2, 8, device='cuda')
+    ops.kv_append(pages, x, x, table, lens)
+    with pytest.raises(RuntimeError, match='k_scale requires a gradient'):
+        ops.KVPages(code, code.clone(), scale.clone().requires_grad_(), scale)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: ops.kv_append(pages, dual(x), x, table, lens), lambda: ops.kv_append(pages, x, dual(x), table, lens),
+                     lambda: ops.paged_attention(dual(q), pages, table, lens), lambda: ops.KVPages(dual(pages.k), pages.v),
+                     lambda: ops.KVPages(code, code.clone(), dual(scale), scale)):
+            with pytest.raises(RuntimeError, match='forward-mode tangent'):
+                call()
+        ops.paged_attention(q, pages, table, lens)                   # without one: as ever
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: ops.paged_attention(t, pages, table, lens), (q,), (q,))
     torch.cuda.synchronize()
