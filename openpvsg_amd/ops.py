@@ -1654,7 +1654,7 @@ class KVPages:
     fixed: for others (a larger pool) make another KVPages."""
 
     __slots__ = ('k', 'v', 'k_scale', 'v_scale', 'dtype', 'device', 'index', 'num_pages', 'heads', 'page_size', 'head_dim', '_struct',
-                 '_axes', '_spans', '_shared')
+                 '_axes', '_spans', '_shared', '_written')
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         for n, t in (('k', k), ('v', v)):
@@ -1701,6 +1701,7 @@ class KVPages:
         self._shared = _rows_meet(at[1] - at[0], self._axes, D * size) or any(_rows_touch(a, self._axes, D * size, *t) for a in at for t in scales) or \
             (scaled and scales[0][0] < scales[1][1] and scales[1][0] < scales[0][1])
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._written = (k, v, k_scale, v_scale) if scaled else (k, v)
         self.dtype, self.device, self.index = k.dtype, k.device, k.get_device()
         self.num_pages, self.heads, self.page_size, self.head_dim = P, H, S, D
         self._struct = _lib.KvPages(k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if scaled else None,
@@ -1825,6 +1826,7 @@ def kv_append(pages, k, v, table, lens, new_lens=None):
         _lib.call('pvsg_kv_append', pages._struct, a, b, _KV_ROW_TYPES[k.dtype], sb, st, sh, table.data_ptr(), row,
                   width, lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, B, T,
                   _stream_ptr())
+    torch._C._increment_version(pages._written)                     # written in place: a backward that saved one of them must notice
     return pages
 
 
@@ -1893,7 +1895,8 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
         if mask.shape[1] and mask.stride(1) != 1:
             mask = mask.contiguous()
         ms, mw = mask.stride(0), mask.shape[1]
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((B, T, HQ, D))
     elif not isinstance(out, torch.Tensor) or out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous() or \
             out.data_ptr() & 15 or out.requires_grad:
@@ -1918,4 +1921,6 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
                   lens.data_ptr(), new_lens.data_ptr() if new_lens is not None else None, mask.data_ptr() if mask is not None else None,
                   ms, mw, B, T, HQ, D ** -0.5 if scale is None else float(scale), 1 if causal else 0, longest,
                   work.data_ptr() if work is not None else None, counters.data_ptr() if nbytes else None, stream)
+    if given:
+        torch._C._increment_version((out,))
     return out

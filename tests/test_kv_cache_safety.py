@@ -179,3 +179,32 @@ def test_derivatives_are_refused(hip_lib):
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda t: ops.paged_attention(t, pages, table, lens), (q,), (q,))
     torch.cuda.synchronize()
+
+
+@gpu
+@pytest.mark.parametrize('dtype', (torch.float32, torch.int8), ids=str)
+def test_writes_raise_the_version_counters(hip_lib, dtype):
+    """a backward pass that saved a tensor of the pool, or an `out`, stops instead of running on what was written since"""
+    from openpvsg_amd import ops
+    pages = ops.KVPages.empty(4, 2, 8, 32, dtype=dtype)
+    table, lens = torch.arange(4, dtype=torch.int32, device='cuda').view(2, 2), torch.full((2,), 3, dtype=torch.int32, device='cuda')
+    x, q = torch.ones(2, 3, 2, 32, device='cuda'), torch.ones(2, 3, 4, 32, device='cuda')
+    written = [t for t in (pages.k, pages.v, pages.k_scale, pages.v_scale) if t is not None]
+    before = [t._version for t in written]
+    ops.kv_append(pages, x, x, table, lens)
+    assert all(t._version > n for t, n in zip(written, before))
+    before = [t._version for t in written]
+    out = torch.empty_like(q)
+    n = out._version
+    ops.kv_read(pages, table, lens, 3), ops.paged_attention(q, pages, table, lens, out=out)
+    assert [t._version for t in written] == before and out._version > n
+    w = torch.ones(32, device='cuda', requires_grad=True)
+    saved = written[-1] if dtype == torch.int8 else pages.v
+    loss = (saved * (w.sum() if dtype == torch.int8 else w)).sum()
+    ops.kv_append(pages, x, x, table, lens)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+    with torch.inference_mode():                                     # tensors that have no counter
+        ops.kv_append(ops.KVPages.empty(4, 2, 8, 32, dtype=dtype), x, x, table, lens)
+        ops.paged_attention(q, pages, table, lens, out=torch.empty_like(q))
+    torch.cuda.synchronize()
