@@ -11,6 +11,7 @@ from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
+INCLUDE = os.path.join(os.path.dirname(HERE), 'include')      # the C ABI: kernels take its structs by value
 LIBDIR = os.path.join(HERE, 'lib')
 OBJDIR = os.path.join(LIBDIR, 'obj')
 LIBNAME = 'libopenpvsg_hip.so'
@@ -46,7 +47,7 @@ def _stale(target, deps):
 
 def build_hip_lib(force=False, verbose=True):
     os.makedirs(OBJDIR, exist_ok=True)
-    headers = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith('.h')]
+    headers = [os.path.join(d, f) for d in (CSRC, INCLUDE) for f in os.listdir(d) if f.endswith('.h')]
     jobs = []
     objs = []
     for src in _sources():
