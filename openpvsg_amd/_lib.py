@@ -235,10 +235,10 @@ _external = {}                             # device -> [handle, event behind the
 
 def _stream_taken(stream, dev):
     """`stream` carries the launches of device `dev` from now on: note whose it is"""
+    if stream not in _torch_owned and torch._C._cuda_getCurrentRawStream(dev) == stream and torch._C._cuda_getCurrentStream(dev)[0] & 1:
+        _torch_owned.add(stream)                       # (a pool stream's id is odd)
     if stream in _torch_owned:
-        return
-    if torch._C._cuda_getCurrentRawStream(dev) == stream and torch._C._cuda_getCurrentStream(dev)[0] & 1:   # a pool stream's id is odd
-        _torch_owned.add(stream)
+        _external.pop(dev, None)                       # the one before is not asked about any more: launches leave no events again
         return
     ent = _external.get(dev)
     if ent is None or ent[0] != stream:
