@@ -228,7 +228,8 @@ except AttributeError:                    # pragma: no cover
 
 # A stream handle may only be asked about while the stream lives: the runtime follows a destroyed one into freed memory.  torch's own
 # streams (the default one and its pools') live as long as the process; a stream that torch was merely handed (an ExternalStream)
-# may be gone by the time the next one takes over, so behind each launch on one an event is left, which outlives it.
+# may be gone by the time the next one takes over, so behind each launch on one an event is left, which outlives it.  Other work on such a
+# stream cannot be seen that way: leaving one for another stream waits for the device.
 _torch_owned = {0}
 _external = {}                             # device -> [handle, event behind the last launch]
 
@@ -290,6 +291,8 @@ def _stream_changed(name, stream, ent):
             '16-bit-MFMA kernels must not share the GPU with other kernels (co-residency corruption, DESIGN.md section 3).  '
             'Keep the backend on one stream per device, or order the streams (wait_stream + synchronize) before switching; '
             'PVSG_MULTI_STREAM=allow disables this check.' % (name, stream, prev))
+    if prev is not None and (mfma16 or ent[1]) and prev not in _torch_owned:
+        torch.cuda.synchronize(_cur_dev())             # what others put there is not known, and it may not be asked: waited for
     _stream_taken(stream, _cur_dev())
     ent[0], ent[1] = stream, mfma16
 
