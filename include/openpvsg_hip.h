@@ -684,7 +684,8 @@ int pvsg_kv_read(const pvsg_kv_pages* pages, void* k_out, void* v_out, int out_t
  * pool's heads (query head j reads key head j / (q_heads / heads)); T <= 32.  Pools: of row_type, or 8-bit; with row_type F32 any.
  * Row t of sequence b sees positions p < lens[b], with causal != 0 only p <= lens[b] - n_b + t, and with padding (bool bytes,
  * (B, padding_width) rows padding_stride apart, nonzero = ignored) only p < padding_width with a zero there.  softmax(scale * q.k) v in f32, rounded
- * once; a row that sees nothing, or past n_b, is zero.  What a row does not see does not reach it, NaN and infinities included.
+ * once (over F16 pools weights below 2^-29 of the row's largest to 2^-40 of it); a row whose weights sum to zero -- that sees nothing, or
+ * only logits of -infinity -- or past n_b is zero.  What a row does not see does not reach it, NaN and infinities included.
  * max_len: the longest cache to plan for (0: what the table holds); longer ones are computed all the same.
  * workspace: pvsg_paged_attention_workspace_bytes of the same arguments (0: none), 16-byte aligned, no initialisation.
  * counters: needed with a workspace: PVSG_PAGED_ATTENTION_COUNTERS words that were zero before the first call that was given them and that no two

@@ -1,6 +1,7 @@
 // Attention of 1..32 new tokens per sequence over a paged key/value pool, split over the cache's length and joined.
 //
-//   o = sum_p softmax(scale * q . k_p) v_p,  one pass over the keys with a running maximum m and sum l per row.
+//   o = sum_p softmax(scale * q . k_p) v_p,  one pass over the keys with a running maximum m and sum l per row; 0 where l is 0: a row
+//   that sees nothing, or only logits of -infinity (which leave m there).
 //
 // The T * (q_heads / kv_heads) query rows that share a key head make 16-row tiles.  A wave walks the cache in tiles of KEYS keys and
 // feeds the matrix cores straight from global memory, with no LDS between: keys are the A operand of S^T = K Q^T (a lane's part of

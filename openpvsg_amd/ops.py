@@ -1866,14 +1866,15 @@ def _paged_attention_counters(device, stream):
 
 
 def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None, causal=True, scale=None, max_len=None, out=None):
-    """Attention of new tokens over the cached keys and values: softmax(scale * q . k) v, in float32, rounded once to q's dtype.
+    """Attention of new tokens over the cached keys and values: softmax(scale * q . k) v, in float32, rounded once to q's dtype
+    (over a float16 pool weights below 2^-29 of a row's largest are held to 2^-40 of it).
 
     q (B, T, q_heads, head_dim), T <= 32, in the pool's dtype, or float32 over any pool, or any of float32 / bfloat16 / float16 over an
     8-bit pool; q_heads a multiple of the pool's heads (shared key heads).  table, lens, new_lens as in kv_append (append first: the new tokens
     see themselves).  Token t of sequence b, at position lens[b] - n + t, sees the positions before lens[b]; with `causal` (default) those
     up to its own; with key_padding_mask (B, M) bool, True = ignored as in torch's attention, and positions from M on ignored too.
-    A row that sees nothing (an empty sequence, a token past n, everything masked) is zero; what is masked never reaches a
-    result, NaN and infinities included.  scale defaults to head_dim ** -0.5.  max_len: the longest cache to plan the split for, if
+    A row whose weights sum to zero is zero: one that sees nothing (an empty sequence, a token past n, everything masked), and one whose
+    logits are all -infinity, where torch's softmax gives NaN.  What is masked never reaches a result, NaN and infinities included.  scale defaults to head_dim ** -0.5.  max_len: the longest cache to plan the split for, if
     the table holds much more (longer ones are computed all the same).  out: (B, T, q_heads, head_dim), contiguous, apart from every input.
     -> (B, T, q_heads, head_dim)"""
     q = _kv_rows(q, 'q', pages, None)

@@ -105,3 +105,36 @@ def test_weights_hold_the_bits_of_f32(hip_lib, row, pool):
         tol = 26 * 2.0 ** -24 * (w[..., None] * x.abs()).sum(0) / w.sum(0)[:, None] + torch.finfo(row).eps / 2 * want.abs() + (2.0 ** -25 if row == torch.float16 else 0.0)
         err = (got[b] - want).abs()
         assert bool((err <= tol).all()), (b, 'worst %.3g of its tolerance' % float((err / tol).max()))
+
+
+@gpu
+@pytest.mark.parametrize('row,pool', ((torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16), (torch.float16, torch.float16),
+                                      (torch.bfloat16, torch.float8_e4m3fn)), ids=lambda t: str(t)[6:])
+@pytest.mark.parametrize('D', (16, 64))
+def test_logits_of_minus_infinity(hip_lib, row, pool, D):
+    """a row that sees only those is zero, split or not; beside finite ones they have no weight; one of +infinity makes the row NaN"""
+    from openpvsg_amd import ops
+    inf = float('inf')
+    for n in (1, 70, 5000):
+        c = Cache(ops, [n] * 4, 1, D, 16, pool, n)
+        q = torch.ones(4, 1, 1, D, dtype=row)
+        p = torch.arange(n)
+
+        def put(b, where, x):
+            page, slot = c.table[b, where // 16].long().cuda(), (where % 16).cuda()
+            if pool == torch.float8_e4m3fn:
+                c.pages.k.view(torch.uint8)[page, :, slot] = torch.full((1, D), 1.0).to(pool).view(torch.uint8).cuda()
+                c.pages.k_scale[page, :, slot] = x
+            else:
+                c.pages.k[page, :, slot] = x
+        put(0, p, -inf)
+        put(1, p[:n // 2], -inf)
+        put(2, p, -inf)
+        put(2, p[n // 3:n // 3 + 1], inf)
+        got = ops.paged_attention(q.cuda(), c.pages, c.dev_table, c.dev_lens).cpu().double()
+        assert not bool(got[0].any())
+        assert bool(got[2].isnan().all())
+        for b, first in ((1, n // 2), (3, 0)):
+            want, size, every, rel = by_weight(q[b, 0, 0].double(), c.rows[0][b][first:, 0], c.rows[1][b][first:, 0], D ** -0.5)
+            tol = (rel + 2.0 ** -22) * size + 2.0 ** -40 * every + torch.finfo(row).eps / 2 * want.abs() + (2.0 ** -25 if row == torch.float16 else 0.0)
+            assert bool(((got[b, 0, 0] - want).abs() <= tol).all()), (n, b)
