@@ -644,7 +644,9 @@ int pvsg_bottleneck_tail_f16x2(const float* mid, const void* w3_packed, const fl
 
 /* ---- paged key/value cache: live video --------------------------------------------------------
  * The reference re-runs its temporal encoder over every frame so far (models/relation_head/transformer.py:26-56 takes the whole
- * (P, T, C) block); with these a call projects only its new frames, appends their keys and values, and attends over the cache.
+ * (P, T, C) block); with these a call projects only its new frames, appends their keys and values, and attends over the cache.  That gives
+ * the newest frames' rows of a layer: the encoder is bidirectional, so the older frames' rows change with each new frame, and a second
+ * layer's cache would have to be made again.
  *
  * A pool holds K and V as (num_pages, heads, page_size, dim): dim dense, the first three axes with strides in ELEMENTS, the same
  * for K and V and multiples of 16 bytes; base addresses 16-byte aligned.  page_size: a power of two in [8, 65536]; dim: a multiple of 16 up
@@ -656,7 +658,8 @@ int pvsg_bottleneck_tail_f16x2(const float* mid, const void* w3_packed, const fl
  * Lengths and page ids live on the device, so they are checked there: a page id outside the pool, or a length past the table, is
  * never followed -- such rows are not written / read as zero / not attended to, and a bit of *faults (may be NULL) is set:
  * 1 append, 2 read, 4 attention.
- * Pages that a sequence appends to belong to it alone; pages that are only read may be in several rows of the table. */
+ * Pages that a sequence appends to belong to it alone; pages that are only read may be in several rows of the table.  What a call writes (the
+ * pool's k, v and scales in append, k_out and v_out, out) shares no memory with itself or with what the call reads. */
 #define PVSG_TYPE_F32 0
 #define PVSG_TYPE_BF16 1
 #define PVSG_TYPE_F16 2

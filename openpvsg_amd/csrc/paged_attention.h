@@ -16,17 +16,17 @@
 // no cache is longer than a few tiles there is nothing to even out, and each has a workgroup of its own and no join.
 //
 // Rounding: 16-bit rows multiply in their own type, exact products in f32 sums; 8-bit codes convert to it exactly and their
-// scales multiply S and P in f32.  P goes to the matrix cores with the bits that f32 has: as three bf16 parts over a bf16 or 8-bit pool,
-// as two f16 parts over a f16 one (see LIFT).  One part alone adds an error as large as the rounding of the result itself; two of bf16
-// hold 16 bits, which shows where values cancel, and save little (100 x up to 5000 x 4 x 128 e4m3, 32 new tokens: 77.4 us, three parts
-// 79.7; 64 x 8192 x 8 heads of 64 int8 110.8 and 116.7; 8 x 65536 bf16 361 both).  f32 rows over a bf16 or 8-bit pool go as three bf16 parts too.  At
+// scales multiply S and P in f32.  P goes to the matrix cores as three bf16 parts over a bf16 or 8-bit pool (the 24 bits of f32), as two f16
+// parts over a f16 one (22, see LIFT).  One part alone adds an error as large as the rounding of the result itself; two of bf16
+// hold 16 bits, which shows where values cancel, and save little (100 x up to 5000 x 4 x 128 e4m3, 32 new tokens: 78.7 us, three parts
+// 79.8; 64 x 8192 x 8 heads of 64 int8 119.1 and 122.8; 8 x 65536 bf16 361 both).  f32 rows over a bf16 or 8-bit pool go as three bf16 parts too.  At
 // the matrix cores' peak three 16-bit products take 3/16 of the time that the f32 ones would.  f32 rows over a f32 or f16 pool run on the f32
 // products.
 //
-// Measured: 8 x 65536 x 8 key heads of 128 bf16 359 us, 5.95 TB/s, bound by HBM; 100 ragged caches of up to 900 x 4 x 128 f32 48 us,
+// Measured: 8 x 65536 x 8 key heads of 128 bf16 360 us, 5.95 TB/s, bound by HBM; 100 ragged caches of up to 900 x 4 x 128 f32 48 us,
 // 3.85 TB/s: a stretch takes 5 us to its first keys (lengths, scan, page ids, queries: waits for memory that depend on each other)
 // and 4 to be joined and counted, and with two workgroups on a CU that is covered in part; 100 of up to 5000 x 4 x 128 e4m3, 32 new
-// tokens, 75 us, 3.6 TB/s, the waves as long in the softmax's instructions as in waits; the smallest call 6.6 us, five such waits.
+// tokens, 76 us, 3.6 TB/s, the waves as long in the softmax's instructions as in waits; the smallest call 6.5 us, five such waits.
 #pragma once
 #include "kv_pages.h"
 
@@ -73,8 +73,8 @@ constexpr bool pa_16bit(int row, int pool) { return row != KV_F32 || pool == KV_
 constexpr int pa_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 // 16-key blocks of a wave's tile.  f32 products take one key at a time, so that a block of theirs is work enough.  Of heads of up to 64
 // in 16 bits there is room for four beside the next tile's, and where the caches are long (`split`: the tiles are shared out) they
-// save waits for memory: 64 x 8192 x 8 heads of 64 int8 122 -> 109 us, 20 ragged ones of up to 3000 18.1 -> 15.7.  Short ones go two blocks at a time,
-// three workgroups to a CU: 100 of up to 900 positions 19.3 us, and 22.3 with four.
+// save waits for memory: 64 x 8192 x 8 heads of 64 int8 130.9 -> 122.8 us, 20 ragged ones of up to 3000 x 8 bf16 19.9 -> 18.6.  Short ones go two
+// blocks at a time, three workgroups to a CU: 100 of up to 900 positions x 8 int8 21.2 us, and 24.7 with four.
 constexpr int pa_blocks(int row, int pool, int dim, int tiles, bool split) {
   return pa_16bit(row, pool) ? (split && tiles == 1 && row != KV_F32 && dim <= 64 ? 4 : 2) : dim <= 32 ? 2 : 1;
 }

@@ -3,12 +3,19 @@
 
 namespace pvsg {
 
-// Caches of up to so many tiles are not split: each has a workgroup of its own.  Measured over 4 .. 800 (sequence, key head)s of bf16
-// heads of 128: at 700 positions (6 tiles) 11.0 - 37.8 us so and 13.5 - 42.8 us split and joined, at 1000 (8) 13.5 - 50 and 13.7 -
-// 53.7, at 1500 (12) 17.6 - 70 and 13.5 - 71: the wait for a tile's memory, 1.2 us, is paid once a tile.
+// Caches of up to so many tiles are not split: each has a workgroup of its own (and waits once a tile for its memory, 1.2 us).  Measured both
+// ways with 4 heads, 2 / 25 / 100 ragged sequences, us split and joined against whole:
+//   f32 over f32, heads of 128 (64 keys a tile: 512 positions)   up to  400  14.5 / 15.8 / 26.3  against 13.9 / 15.0 / 26.2,  700  14.8 / 16.7 / 41.4  against 19.3 / 20.3 / 43.8
+//   bf16 over bf16, heads of 128 (128 keys: 1024 positions)      up to  700  11.9 / 13.2 / 23.6  against 11.1 / 12.2 / 21.1, 1500  12.5 / 16.3 / 42.1  against 17.8 / 18.9 / 45.5
+//   f32 over e4m3, heads of 128 (128 keys)                       up to 1000  13.7 / 14.8 / 22.5  against 13.1 / 14.1 / 20.4, 1500  13.8 / 15.3 / 25.7  against 17.0 / 18.1 / 27.9
+//   bf16 over e4m3, heads of 64 (128 keys)                       up to 1000  11.8 / 12.2 / 19.2  against 11.4 / 11.8 / 16.1, 1500  12.0 / 12.9 / 20.6  against 15.0 / 15.7 / 20.8
+//   f32 over f32, heads of 32 (128 keys)                         up to 1000  12.5 / 13.6 / 21.3  against 12.0 / 12.8 / 19.5, 1500  12.7 / 13.9 / 25.2  against 15.9 / 16.8 / 25.6
+//   16 new tokens, bf16 over bf16, heads of 128                  up to 1000  15.7 / 17.3 / 36.1  against 14.2 / 15.3 / 31.4, 1500  15.8 / 18.3 / 47.4  against 18.3 / 19.4 / 47.4
 constexpr int PA_SHORT = 8;
 
-// 16-row tiles a wave carries: two where there are more rows than one tile holds and the accumulators of two fit
+// 16-row tiles a wave carries: two where there are more rows than one tile holds and the accumulators of two (of f32 rows: three-part queries
+// or single columns of two) fit.  Rows past that walk the cache again: 100 x up to 5000 x 4 x 128, 16 and 32 new tokens, f32 over f32 211 and
+// 324 us, over bf16 116 and 173, over e4m3 72 and 102.
 static int pa_tiles(int rows, int dim, int row_type) { return rows > 16 && dim <= (row_type == KV_F32 ? 64 : 128) ? 2 : 1; }
 
 // How the work is shared out: rows of a tile group, groups, and how many workgroups take equal stretches (0: one each)

@@ -1578,7 +1578,7 @@ conv3x3s2_bf16x3_supported = conv3x3_bf16x3_supported
 
 # ---- paged key/value cache (csrc/kv_cache.hip, csrc/paged_attention.h) ------------------------------------------------------
 # A live video hands over 1..32 new frames at a time.  Their keys and values are appended to pages that the video owns, and the
-# new frames' queries attend over everything cached: no frame is projected twice.  Lengths and page tables stay on the
+# new frames' queries attend over everything cached: no frame's keys and values are projected twice.  Lengths and page tables stay on the
 # device, so a step is a fixed set of launches (graph-capturable); what they may point at is checked there.
 _KV_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3, torch.int8: 4}
 _KV_ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
