@@ -1710,12 +1710,14 @@ class KVPages:
 
     def __setattr__(self, name, value):
         # the kernels go by the addresses taken when the pool was made, and its tensors are kept alive for them
-        if hasattr(self, '_struct'):
+        if name in KVPages.__slots__ and hasattr(self, '_struct'):
             raise AttributeError('KVPages: %s is fixed once the pool is made; make another KVPages' % name)
         object.__setattr__(self, name, value)
 
     def __delattr__(self, name):
-        raise AttributeError('KVPages: %s is fixed once the pool is made' % name)
+        if name in KVPages.__slots__:
+            raise AttributeError('KVPages: %s is fixed once the pool is made' % name)
+        object.__delattr__(self, name)
 
     @classmethod
     def empty(cls, num_pages, heads, page_size, head_dim, dtype=torch.float32, device='cuda'):

@@ -47,6 +47,21 @@ def test_a_pools_tensors_are_fixed():
     assert pages.k.shape == (2, 1, 8, 16)
 
 
+def test_a_subclass_keeps_attributes_of_its_own():
+    from openpvsg_amd import _lib, ops
+
+    class Video(ops.KVPages):
+        pass
+    pages = Video.__new__(Video)
+    pages._struct = _lib.KvPages()
+    pages.name = 'a'
+    pages.name = 'b'
+    assert pages.name == 'b'
+    del pages.name
+    with pytest.raises(AttributeError, match='fixed'):
+        pages.k = None
+
+
 def test_a_tangent_is_seen():
     from torch.autograd import forward_ad
 
