@@ -1779,17 +1779,15 @@ def _kv_rows(t, name, pages, heads):
 
 
 def _kv_meets(out, pages, *others):
-    """whether the dense tensor `out` shares memory with the pool or another input"""
+    """whether the dense tensor `out` shares memory with the pool or another input, (tensor or None, bytes from its first element on)"""
     lo = out.data_ptr()
     hi = lo + out.numel() * out.element_size()
-    size = pages.head_dim * pages.k.element_size()
-    if any(_rows_touch(a, pages._axes, size, lo, hi) for a, _ in pages._spans[:2]) or any(lo < b and a < hi for a, b in pages._spans[2:]):
-        return True
-    for t in others:
-        if t is not None and t.numel():
-            a = t.data_ptr()
-            if lo < a + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() and a < hi:
-                return True
+    for i, (a, b) in enumerate(pages._spans):
+        if a < hi and lo < b and (i > 1 or _rows_touch(a, pages._axes, pages.head_dim * pages.k.element_size(), lo, hi)):
+            return True
+    for t, n in others:
+        if t is not None and n and lo - n < t.data_ptr() < hi:
+            return True
     return False
 
 
@@ -1907,7 +1905,7 @@ def paged_attention(q, pages, table, lens, new_lens=None, key_padding_mask=None,
     elif out.data_ptr() < q.data_ptr() + (sum((n - 1) * s for n, s in zip(q.shape, q.stride())) + 1) * q.element_size() and \
             q.data_ptr() < out.data_ptr() + out.numel() * out.element_size() and out.numel():
         raise RuntimeError('paged_attention: out overlaps q')
-    elif out.numel() and _kv_meets(out, pages, table, lens, new_lens, mask):
+    elif out.numel() and _kv_meets(out, pages, (table, ((B - 1) * table_row + width) * 4), (lens, B * 4), (new_lens, B * 4), (mask, mw and (B - 1) * ms + mw)):
         raise RuntimeError('paged_attention: out overlaps the pool, the table, the lengths or the mask')
     if mask is not None and mw == 0:
         return out.zero_()

@@ -138,3 +138,23 @@ def test_logits_of_minus_infinity(hip_lib, row, pool, D):
             want, size, every, rel = by_weight(q[b, 0, 0].double(), c.rows[0][b][first:, 0], c.rows[1][b][first:, 0], D ** -0.5)
             tol = (rel + 2.0 ** -22) * size + 2.0 ** -40 * every + torch.finfo(row).eps / 2 * want.abs() + (2.0 ** -25 if row == torch.float16 else 0.0)
             assert bool(((got[b, 0, 0] - want).abs() <= tol).all()), (n, b)
+
+
+@gpu
+@pytest.mark.parametrize('row,pool', ((torch.float16, torch.float16), (torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32)), ids=lambda t: str(t)[6:])
+def test_logits_past_what_f32_counts_by_ones(hip_lib, row, pool):
+    """logits of some 10^7, far apart: the largest key alone, also where f32 cannot hold the maximum less a small number"""
+    from openpvsg_amd import ops
+    D = 64
+    for n in (5, 300, 3000):
+        c = Cache(ops, [n], 1, D, 16, pool, n)
+        p = torch.arange(n)
+        page, slot = c.table[0, p // 16].long().cuda(), (p % 16).cuda()
+        size = torch.full((n,), 1000.0)
+        best = torch.randint(0, n, (1,), generator=c.g)
+        size[best] = 2048.0
+        c.pages.k[page, :, slot] = (size[:, None, None] * torch.ones(n, 1, D)).to(pool).cuda()
+        q = torch.full((1, 2, 1, D), 2048.0, dtype=row)
+        got = ops.paged_attention(q.cuda(), c.pages, c.dev_table, c.dev_lens, causal=False).cpu()
+        # every other weight is exp(-1e7) = 0, the largest 1: the value itself
+        assert torch.equal(got.double(), c.rows[1][0][best].expand(2, 1, D)[None].reshape(1, 2, 1, D)), n
