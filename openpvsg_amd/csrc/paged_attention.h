@@ -19,7 +19,8 @@
 // scales multiply S and P in f32.  P goes to the matrix cores as three bf16 parts over a bf16 or 8-bit pool (the 24 bits of f32), as two f16
 // parts over a f16 one (22, see LIFT).  One part alone adds an error as large as the rounding of the result itself; two of bf16
 // hold 16 bits, which shows where values cancel, and save little (100 x up to 5000 x 4 x 128 e4m3, 32 new tokens: 78.7 us, three parts
-// 79.8; 64 x 8192 x 8 heads of 64 int8 119.1 and 122.8; 8 x 65536 bf16 361 both).  f32 rows over a bf16 or 8-bit pool go as three bf16 parts too.  At
+// 79.8; 64 x 8192 x 8 heads of 64 int8 119.1 and 122.8; 8 x 65536 bf16 361 both).  (P carries the scale of
+// V's codes: rows whose scale is below 2^-100 lose bits, since bf16 ends at 2^-133.)  f32 rows over a bf16 or 8-bit pool go as three bf16 parts too.  At
 // the matrix cores' peak three 16-bit products take 3/16 of the time that the f32 ones would.  f32 rows over a f32 or f16 pool run on the f32
 // products.
 //
